@@ -207,6 +207,54 @@ m3_status m3_mixer_step_conv(const m3_mixer_dims *d, const m3_conv1d *conv, cons
                              m3_ssm_state *state, m3_ssm_state_factored *factored, void *out,
                              void *stream);
 
+/* What stands between two blocks of a residual stack, in one pass over its
+ * rows:
+ *     n            = post_weight x rsqrt(mean(x^2) + eps)   (x without post_norm)
+ *     residual_out = residual + scale act(gate) n
+ *     y            = pre_weight residual_out rsqrt(mean(residual_out^2) + eps)
+ * -- the norm after a block with its gate and residual scale, the residual
+ * add, and the norm before the next block.  No reference counterpart as one
+ * call (RmsNorm::apply src/nn/norm.rs:95-105, HybridLayer's residual add
+ * src/models/hybrid.rs:446-456).  The arithmetic is f32; y follows from the
+ * unrounded residual_out. */
+typedef enum m3_gate_activation {
+    M3_GATE_NONE = 0, M3_GATE_SILU = 1, M3_GATE_SIGMOID = 2
+} m3_gate_activation;
+
+typedef struct m3_block_norm_args {
+    size_t rows, dim;          /* dim up to 32768, else M3_ERR_UNSUPPORTED */
+    int32_t dtype;             /* m3_dtype of x, gate and y */
+    int32_t residual_dtype;    /* of residual and residual_out: dtype or M3_F32 */
+    int32_t post_norm;
+    int32_t activation;        /* m3_gate_activation */
+    float eps;
+    const void *x;             /* [rows, dim] */
+    const void *residual;      /* [rows, dim] */
+    const void *gate;          /* rows gate_stride elements apart, or NULL (no gate) */
+    size_t gate_stride;
+    const float *post_weight;  /* [dim], or NULL (ones) */
+    const float *scale;        /* [dim], or NULL (ones) */
+    const float *pre_weight;   /* [dim], or NULL (ones) */
+} m3_block_norm_args;
+
+/* residual_out may be residual; y may be x, or NULL (no norm after the add). */
+m3_status m3_block_norm(const m3_block_norm_args *a, void *residual_out, void *y, void *stream);
+
+/* Gradients of m3_block_norm.  dresidual_out and dy (either may be NULL: zero)
+ * are given; dx, dresidual and, with a gate, dgate [rows, dim] (contiguous) are
+ * written, and the column sums dpost_weight, dscale and dpre_weight [dim]
+ * unless NULL (summed in a fixed order).  dresidual may be dresidual_out, dx may
+ * be dy.  The workspace holds m3_block_norm_backward_workspace_bytes. */
+typedef struct m3_block_norm_grads {
+    const void *dresidual_out, *dy;
+    void *dx, *dresidual, *dgate;
+    float *dpost_weight, *dscale, *dpre_weight;
+} m3_block_norm_grads;
+
+size_t m3_block_norm_backward_workspace_bytes(const m3_block_norm_args *a);
+m3_status m3_block_norm_backward(const m3_block_norm_args *a, const m3_block_norm_grads *grads,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+
 /* out[i] = table[ids[i]] for bf16 rows of dim (table [vocab, dim]).  The
  * ids live on the device, so they are not checked on the host: an id outside
  * [0, vocab) reads nothing and yields a zero row. */

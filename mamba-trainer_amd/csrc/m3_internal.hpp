@@ -231,6 +231,27 @@ hipError_t launch_mixer_prologue(const PrologueLaunch &a, hipStream_t s);
 hipError_t launch_mixer_gate(size_t tokens, size_t d_inner, const void *y, const void *z,
                              size_t z_stride, const float *norm_w, float eps, void *out,
                              hipStream_t s);
+// The norms, gate, scale and residual add between two blocks, and their
+// gradients (block_norm.hip).
+struct BlockNormLaunch {
+    size_t rows, dim, gate_stride;
+    int dtype, residual_dtype;      // m3_dtype; the residual's is the same or M3_F32
+    int post_norm, act;             // act: m3_gate_activation
+    float eps;
+    const void *x, *residual, *gate;          // gate null: none
+    const float *post_w, *scale, *pre_w;      // [dim] or null (ones)
+    void *residual_out, *y;                   // y null: no norm after the add
+};
+struct BlockNormGrads {
+    const void *dres, *dy;          // of residual_out and y; either may be null
+    void *dx, *dresidual, *dgate;
+    float *dpost_w, *dscale, *dpre_w;   // null: not wanted
+};
+constexpr size_t kBlockNormMaxDim = 32768;
+hipError_t launch_block_norm(const BlockNormLaunch &a, hipStream_t s);
+size_t block_norm_backward_workspace(const BlockNormLaunch &a);
+hipError_t launch_block_norm_backward(const BlockNormLaunch &a, const BlockNormGrads &g, void *workspace,
+                                      hipStream_t s);
 // out[i] = table[ids[i]], bf16 rows of dim (zero rows for ids outside vocab).
 hipError_t launch_embedding(size_t n, size_t dim, const int32_t *ids, size_t vocab, const void *table,
                             void *out, hipStream_t s);

@@ -370,6 +370,73 @@ m3_status m3_mixer_step_conv(const m3_mixer_dims *d, const m3_conv1d *conv, cons
                            post_norm_weight, post_norm_eps, state, factored, out, stream);
 }
 
+namespace {
+m3_status block_norm_args(const m3_block_norm_args *a, m3::BlockNormLaunch &l) {
+    if (a == nullptr) return m3::api_fail(M3_ERR_ARGUMENT, "block norm arguments are NULL");
+    if (a->dim == 0) return m3::api_fail(M3_ERR_SHAPE, "a block norm over an empty axis");
+    if (a->dim > m3::kBlockNormMaxDim || a->rows >= size_t(1) << 31)
+        return m3::api_fail(M3_ERR_UNSUPPORTED, "a block norm takes rows of up to %zu values, below 2^31 of them "
+                            "(got %zu x %zu)", m3::kBlockNormMaxDim, a->rows, a->dim);
+    for (const int32_t d : {a->dtype, a->residual_dtype})
+        if (d != M3_F32 && d != M3_BF16 && d != M3_F16)
+            return m3::api_fail(M3_ERR_ARGUMENT, "unknown dtype %d", static_cast<int>(d));
+    if (a->residual_dtype != a->dtype && a->residual_dtype != M3_F32)
+        return m3::api_fail(M3_ERR_UNSUPPORTED, "the residual stream is in x's type or in f32");
+    if (a->activation < M3_GATE_NONE || a->activation > M3_GATE_SIGMOID)
+        return m3::api_fail(M3_ERR_ARGUMENT, "unknown gate activation %d", static_cast<int>(a->activation));
+    if (!(a->eps >= 0.0f)) return m3::api_fail(M3_ERR_CONFIG, "block norm eps must be non-negative");
+    if (a->gate != nullptr && a->gate_stride < a->dim)
+        return m3::api_fail(M3_ERR_SHAPE, "gate rows (%zu apart) are shorter than the row (%zu)", a->gate_stride,
+                            a->dim);
+    if (a->rows > 0 && (a->x == nullptr || a->residual == nullptr))
+        return m3::api_fail(M3_ERR_ARGUMENT, "x and residual are required");
+    l = m3::BlockNormLaunch{};
+    l.rows = a->rows; l.dim = a->dim; l.gate_stride = a->gate_stride;
+    l.dtype = a->dtype; l.residual_dtype = a->residual_dtype;
+    l.post_norm = a->post_norm; l.act = a->activation; l.eps = a->eps;
+    l.x = a->x; l.residual = a->residual; l.gate = a->gate;
+    l.post_w = a->post_weight; l.scale = a->scale; l.pre_w = a->pre_weight;
+    return M3_OK;
+}
+}  // namespace
+
+m3_status m3_block_norm(const m3_block_norm_args *a, void *residual_out, void *y, void *stream) {
+    m3::BlockNormLaunch l;
+    const m3_status st = block_norm_args(a, l);
+    if (st != M3_OK) return st;
+    if (a->rows == 0) return m3::api_ok();
+    if (residual_out == nullptr) return m3::api_fail(M3_ERR_ARGUMENT, "residual_out is required");
+    l.residual_out = residual_out;
+    l.y = y;
+    return launched(m3::launch_block_norm(l, as_stream(stream)), "block norm launch");
+}
+
+size_t m3_block_norm_backward_workspace_bytes(const m3_block_norm_args *a) {
+    if (a == nullptr || a->dim == 0 || a->dim > m3::kBlockNormMaxDim) return 0;
+    m3::BlockNormLaunch l{};
+    l.rows = a->rows;
+    l.dim = a->dim;
+    return m3::block_norm_backward_workspace(l);
+}
+
+m3_status m3_block_norm_backward(const m3_block_norm_args *a, const m3_block_norm_grads *g, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    m3::BlockNormLaunch l;
+    const m3_status st = block_norm_args(a, l);
+    if (st != M3_OK) return st;
+    if (g == nullptr) return m3::api_fail(M3_ERR_ARGUMENT, "block norm gradients are NULL");
+    if (a->rows > 0 && (g->dx == nullptr || g->dresidual == nullptr || (a->gate != nullptr && g->dgate == nullptr)))
+        return m3::api_fail(M3_ERR_ARGUMENT, "dx, dresidual and, with a gate, dgate are required");
+    const size_t need = m3::block_norm_backward_workspace(l);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return m3::api_fail(M3_ERR_ARGUMENT, "the workspace holds %zu bytes of the %zu needed",
+                            workspace == nullptr ? size_t(0) : workspace_bytes, need);
+    const m3::BlockNormGrads gl{g->dresidual_out, g->dy, g->dx, g->dresidual, g->dgate,
+                                g->dpost_weight, g->dscale, g->dpre_weight};
+    return launched(m3::launch_block_norm_backward(l, gl, workspace, as_stream(stream)),
+                    "block norm backward launch", a->rows > 0 ? 2 : 1);
+}
+
 m3_status m3_embedding_lookup(size_t n, size_t dim, const int32_t *ids, size_t vocab,
                               const void *table, void *out, void *stream) {
     if (dim == 0 || vocab == 0) return m3::api_fail(M3_ERR_SHAPE, "empty embedding table");

@@ -101,6 +101,34 @@ class Conv1dC(C.Structure):
                 ("history", _P), ("new_history", _P)]
 
 
+class DeltaInputsC(C.Structure):
+    """m3_delta_inputs (mamba3_delta.h)."""
+    _fields_ = [("batch", _Z), ("seq", _Z), ("heads", _Z), ("groups", _Z), ("head_dim", _Z),
+                ("d_state", _Z), ("dtype", C.c_int32), ("q", _P), ("k", _P), ("v", _P),
+                ("q_stride", _Z), ("k_stride", _Z), ("v_stride", _Z), ("g", _P), ("beta", _P),
+                ("lengths", _P), ("state", _P), ("scale", C.c_float), ("qk_norm", C.c_int32),
+                ("workspace", _P), ("workspace_bytes", _Z)]
+
+
+class DeltaGradsC(C.Structure):
+    """m3_delta_grads (mamba3_delta.h)."""
+    _fields_ = [(n, _P) for n in ("dy", "dstate", "dq", "dk", "dv", "dg", "dbeta", "dstate0")]
+
+
+class BlockNormC(C.Structure):
+    """m3_block_norm_args (mamba3_mixer.h)."""
+    _fields_ = [("rows", _Z), ("dim", _Z), ("dtype", C.c_int32), ("residual_dtype", C.c_int32),
+                ("post_norm", C.c_int32), ("activation", C.c_int32), ("eps", C.c_float),
+                ("x", _P), ("residual", _P), ("gate", _P), ("gate_stride", _Z),
+                ("post_weight", _P), ("scale", _P), ("pre_weight", _P)]
+
+
+class BlockNormGradsC(C.Structure):
+    """m3_block_norm_grads (mamba3_mixer.h)."""
+    _fields_ = [(n, _P) for n in ("dresidual_out", "dy", "dx", "dresidual", "dgate",
+                                  "dpost_weight", "dscale", "dpre_weight")]
+
+
 SIGNATURES = {
     "m3_config_default": (C.c_int, [C.POINTER(SsmConfigC)]),
     "m3_config_validate": (C.c_int, [C.POINTER(SsmConfigC)]),
@@ -143,6 +171,15 @@ SIGNATURES = {
                       [C.POINTER(SsmStateC), C.POINTER(SsmStateFactoredC), _P, _P]),
     "m3_mixer_step_conv": (C.c_int, [C.POINTER(MixerDimsC), C.POINTER(Conv1dC)] + [_P] * 8 +
                            [C.c_float, C.POINTER(SsmStateC), C.POINTER(SsmStateFactoredC), _P, _P]),
+    "m3_block_norm": (C.c_int, [C.POINTER(BlockNormC), _P, _P, _P]),
+    "m3_block_norm_backward_workspace_bytes": (_Z, [C.POINTER(BlockNormC)]),
+    "m3_block_norm_backward": (C.c_int, [C.POINTER(BlockNormC), C.POINTER(BlockNormGradsC), _P, _Z, _P]),
+    # mamba3_delta.h
+    "m3_delta_rule_workspace_bytes": (_Z, [C.POINTER(DeltaInputsC)]),
+    "m3_delta_rule": (C.c_int, [C.POINTER(DeltaInputsC), _P, _P, _P]),
+    "m3_delta_step": (C.c_int, [C.POINTER(DeltaInputsC), _P, _P, _P]),
+    "m3_delta_rule_backward_workspace_bytes": (_Z, [C.POINTER(DeltaInputsC)]),
+    "m3_delta_rule_backward": (C.c_int, [C.POINTER(DeltaInputsC), C.POINTER(DeltaGradsC), _P]),
     # mamba3_checkpoint.h
     "m3_checkpoint_load": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "m3_state_dict_load": (C.c_int, [C.c_char_p, C.POINTER(_P)]),

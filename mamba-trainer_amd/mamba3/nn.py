@@ -9,6 +9,7 @@ are held on the device; every computation runs in libmamba3_hip.so.
 from __future__ import annotations
 
 import ctypes as C
+import dataclasses
 import math
 from typing import Optional
 
@@ -196,6 +197,167 @@ def linear_normed(linear, x: torch.Tensor, norm) -> torch.Tensor:
     if isinstance(linear, Linear):
         return linear.apply_normed(x, norm)
     return linear.apply(norm.apply(x))
+
+
+_TYPES = {torch.float32: _lib.M3_F32, torch.bfloat16: _lib.M3_BF16, torch.float16: _lib.M3_F16}
+_ACTIVATIONS = {"none": 0, "silu": 1, "sigmoid": 2}
+
+
+def _gate_rows(gate: torch.Tensor, shape) -> tuple:
+    """A gate read in place: (tensor, elements between its rows).  Rows that are
+    evenly spaced and contiguous (columns of a projection) stay where they
+    are; anything else is copied."""
+    if tuple(gate.shape) != tuple(shape):
+        raise ShapeError(f"shape error: gate has shape {list(gate.shape)}, expected {list(shape)}")
+    stride = gate.shape[-1]
+    ok = gate.stride(-1) == 1
+    if gate.dim() > 1:
+        stride = gate.stride(-2)
+        want = stride
+        for size, st in zip(reversed(gate.shape[:-1]), reversed(gate.stride()[:-1])):
+            ok = ok and (size == 1 or st == want)
+            want *= size
+    if gate.numel() > 0 and (not ok or stride < gate.shape[-1]):
+        gate = gate.contiguous()
+        stride = gate.shape[-1]
+    return gate, max(stride, gate.shape[-1])
+
+
+def _block_norm_args(x, residual, post_weight, gate, scale, pre_weight, eps, activation, post_norm):
+    """The checked arguments of m3_block_norm, and the tensors they point into."""
+    if not x.is_cuda:
+        raise ArgumentError(f"x must be a ROCm device tensor (got {x.device}); there is no CPU path")
+    if x.dtype not in _TYPES:
+        raise UnsupportedError(f"unsupported: storage dtype {x.dtype}; use float32, bfloat16 or float16")
+    if activation not in _ACTIVATIONS:
+        raise ArgumentError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if x.dim() == 0:
+        raise ShapeError("shape error: a block norm takes rows, got a scalar")
+    dim = x.shape[-1]
+    if tuple(residual.shape) != tuple(x.shape):
+        raise ShapeError(f"shape error: residual has shape {list(residual.shape)}, expected "
+                         f"{list(x.shape)}")
+    if residual.dtype not in (x.dtype, torch.float32):
+        raise UnsupportedError("unsupported: the residual stream is in x's type or in float32, got "
+                               f"{residual.dtype}")
+    for t, what in ((residual, "residual"), (gate, "gate"), (post_weight, "post_weight"),
+                    (scale, "scale"), (pre_weight, "pre_weight")):
+        if t is not None and t.device != x.device:
+            raise ArgumentError(f"{what} is on {t.device}, x on {x.device}")
+    x, residual = x.contiguous(), residual.contiguous()
+    gate_stride = dim
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise ShapeError(f"shape error: gate is {gate.dtype} but x is {x.dtype}")
+        gate, gate_stride = _gate_rows(gate, x.shape)
+    weights = []
+    for t, what in ((post_weight, "post_weight"), (scale, "scale"), (pre_weight, "pre_weight")):
+        if t is not None:
+            if tuple(t.shape) != (dim,):
+                raise ShapeError(f"shape error: {what} has shape {list(t.shape)}, expected [{dim}]")
+            t = t.float().contiguous()
+        weights.append(t)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    rows = x.numel() // dim if dim else 0
+    args = _lib.BlockNormC(rows, dim, _TYPES[x.dtype], _TYPES[residual.dtype], int(bool(post_norm)),
+                           _ACTIVATIONS[activation], float(eps), x.data_ptr(), residual.data_ptr(),
+                           ptr(gate), gate_stride, *(ptr(t) for t in weights))
+    return args, (x, residual, gate, *weights)
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight=None, gate=None, scale=None,
+               pre_weight=None, eps: float = 1e-5, activation: str = "silu", post_norm: bool = True,
+               normed: bool = True):
+    """What stands between two blocks, in one pass over the rows: with
+    n = RMSNorm(x) * post_weight (n = x without post_norm),
+
+        residual' = residual + scale * act(gate) * n
+        y = RMSNorm(residual') * pre_weight
+
+    Returns (residual', y); y is None without `normed`.  x, gate and y share a
+    type; residual and residual' have x's or float32.  Weights are f32 [dim]
+    and may be None (ones); gate None is no gate, activation "none" a plain
+    factor.  A gate whose rows are columns of a wider row is read in place.
+    Differentiable."""
+    tensors = (x, residual, gate, post_weight, scale, pre_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        r, y = _BlockNormFn.apply((eps, activation, post_norm, normed), *tensors)
+        return r, y
+    return _block_norm_forward(tensors, eps, activation, post_norm, normed)
+
+
+def _block_norm_forward(tensors, eps, activation, post_norm, normed):
+    x, residual, gate, post_weight, scale, pre_weight = tensors
+    args, keep = _block_norm_args(x, residual, post_weight, gate, scale, pre_weight, eps, activation,
+                                  post_norm)
+    x, residual = keep[0], keep[1]
+    r = torch.empty_like(residual)
+    y = torch.empty_like(x) if normed else None
+    _lib.check(_lib.lib().m3_block_norm(C.byref(args), r.data_ptr(), None if y is None else y.data_ptr(),
+                                        _stream(x)))
+    return r, y
+
+
+@dataclasses.dataclass
+class BlockNormGrads:
+    """Gradients of block_norm's inputs (None where the input is absent)."""
+    x: torch.Tensor
+    residual: torch.Tensor
+    gate: Optional[torch.Tensor]
+    post_weight: Optional[torch.Tensor]
+    scale: Optional[torch.Tensor]
+    pre_weight: Optional[torch.Tensor]
+
+
+def block_norm_backward(x, residual, dresidual, dy, *, post_weight=None, gate=None, scale=None,
+                        pre_weight=None, eps: float = 1e-5, activation: str = "silu",
+                        post_norm: bool = True) -> BlockNormGrads:
+    """Gradients of block_norm for dL/dresidual' = dresidual and dL/dy = dy
+    (either may be None: zero)."""
+    args, keep = _block_norm_args(x, residual, post_weight, gate, scale, pre_weight, eps, activation,
+                                  post_norm)
+    x, residual, gate = keep[:3]
+    douts = []
+    for t, like, what in ((dresidual, residual, "dresidual"), (dy, x, "dy")):
+        if t is not None:
+            if t.device != x.device:
+                raise ArgumentError(f"{what} is on {t.device}, x on {x.device}")
+            if tuple(t.shape) != tuple(like.shape):
+                raise ShapeError(f"shape error: {what} has shape {list(t.shape)}, expected "
+                                 f"{list(like.shape)}")
+            t = t.to(like.dtype).contiguous()
+        douts.append(t)
+    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device)
+    g = BlockNormGrads(new(x), new(residual), new(gate), *(new(t) for t in keep[3:]))
+    need = int(_lib.lib().m3_block_norm_backward_workspace_bytes(C.byref(args)))
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    gc = _lib.BlockNormGradsC(ptr(douts[0]), ptr(douts[1]), *(ptr(t) for t in (
+        g.x, g.residual, g.gate, g.post_weight, g.scale, g.pre_weight)))
+    _lib.check(_lib.lib().m3_block_norm_backward(C.byref(args), C.byref(gc), ws.data_ptr(), ws.numel(),
+                                                 _stream(x)))
+    return g
+
+
+class _BlockNormFn(torch.autograd.Function):
+    """block_norm as one differentiable node."""
+
+    @staticmethod
+    def forward(ctx, cfg, *tensors):
+        ctx.cfg = cfg
+        ctx.save_for_backward(*tensors)
+        ctx.set_materialize_grads(False)
+        return _block_norm_forward(tensors, *cfg)
+
+    @staticmethod
+    def backward(ctx, dres, dy):
+        x, residual, gate, post_weight, scale, pre_weight = ctx.saved_tensors
+        eps, activation, post_norm, _ = ctx.cfg
+        g = block_norm_backward(x, residual, dres, dy, post_weight=post_weight, gate=gate, scale=scale,
+                                pre_weight=pre_weight, eps=eps, activation=activation,
+                                post_norm=post_norm)
+        out = (g.x, g.residual, g.gate, g.post_weight, g.scale, g.pre_weight)
+        return (None, *(None if t is None else d.to(t.dtype) for t, d in zip(ctx.saved_tensors, out)))
 
 
 class Embedding:
