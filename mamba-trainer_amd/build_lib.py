@@ -23,7 +23,7 @@ SOURCES = ["m3_api.cpp", "m3_mixer_api.cpp", "linear.cpp", "checkpoint.cpp", "ss
            "ssd_scan_fast.hip", "ssd_scan_chunked.hip", "ssd_scan_backward.hip",
            "ssd_scan_backward_generic.hip", "scan_pad.hip", "decode_step.hip", "mfma_selftest.hip",
            "mixer_ops.hip", "skinny_gemm.hip", "few_rows.hip", "m3_delta_api.cpp",
-           "delta_recur.hip", "delta_backward.hip", "block_norm.hip"]
+           "delta_recur.hip", "delta_chunk.hip", "delta_backward.hip", "block_norm.hip"]
 ARCH = "gfx950"
 # Packed-FP32 instructions stay off: hipcc derives them from plain float code
 # and some forms have been unreliable; scalar FP32 is used instead.

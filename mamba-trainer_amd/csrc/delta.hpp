@@ -2,6 +2,8 @@
 // storage types (bf16, f16, f32; all arithmetic is in f32 or wider).
 #pragma once
 
+#include <type_traits>
+
 #include "m3_device.hpp"
 
 namespace m3 {
@@ -31,6 +33,12 @@ constexpr size_t kDeltaMaxState = 256;
 
 // The recurrence token by token with the state in registers (delta_recur.hip).
 hipError_t launch_delta_recur(const DeltaLaunch &a, hipStream_t s);
+
+// Chunk by chunk on the MFMA (delta_chunk.hip): whether a window takes this
+// form, the workspace it needs, and the launch.
+bool delta_chunk_wanted(const DeltaLaunch &a);
+size_t delta_chunk_workspace(const DeltaLaunch &a);
+hipError_t launch_delta_chunk(const DeltaLaunch &a, void *workspace, hipStream_t s, int &launches);
 
 size_t delta_backward_workspace(const DeltaLaunch &a);
 hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void *workspace,

@@ -1,0 +1,243 @@
+// The chunked form of the gated delta rule: what its forward and backward
+// kernels share.
+//
+// A chunk is C = 64 tokens.  With G the running sum of its log decays (taken in
+// f64, so that a difference of two is exact to f32 however large they are),
+// D_ij = exp(G_i - G_j), M_ij = D_ij k_i.k_j (j < i) and T = (I + M diag(beta))^-1:
+//   R = V - diag(exp G) K S0^T        what the state before the chunk leaves of v
+//   E = T R                           each token's prediction error
+//   Y = scale (diag(exp G) Q S0^T + (tril(Q K^T) . D) diag(beta) E)
+//   S1 = exp(G_C) S0 + (diag(beta exp(G_C - G)) E)^T K
+// T depends on the keys alone, so every chunk's is formed at once (delta_prep);
+// only S passes from chunk to chunk.
+//
+// Numbers.  Products run on the bf16 MFMA.  An f32 operand goes in as a sum of
+// bf16 parts, x = x0 + x1 + x2 (each rounding what the ones before left), which
+// is exact to 24 bits in three and to 16 in two; products of parts whose order
+// falls below the last are left out.  bf16 inputs are one part, f16 two, f32
+// three.  Row factors (decay, beta, the unit-length norm's) multiply f32
+// accumulators, never an operand before its rounding.
+//
+// Registers.  A 16x16 accumulator tile holds rows 4g + r in lane group g, and a
+// 16x16x32 operand takes eight k a lane in any order that both operands share:
+// two accumulator tiles (rows 4g .. 4g+3 of each) are an operand as they lie.
+// So a wave that owns 16 columns of P takes its columns of S, R and E from
+// product to product in registers; what it reads from LDS are the chunk's own
+// operands, stored in that order (`slot`).
+#pragma once
+
+#include "delta.hpp"
+
+namespace m3 {
+namespace delta {
+
+constexpr int kC = 64;          // tokens of a chunk
+constexpr int kTri = 6;         // 16 x 32 blocks of a triangular 64 x 64 operand
+
+// bf16 parts of a stored value.
+template <typename T> struct Parts;
+template <> struct Parts<bf16_t> { static constexpr int in = 1, out = 2; };
+template <> struct Parts<f16_t> { static constexpr int in = 2, out = 2; };
+template <> struct Parts<float> { static constexpr int in = 3, out = 3; };
+constexpr int kNP = 3;          // of an f32 value on the way of the state
+
+// Where column n of a row lies in LDS: the eight k-slots of a lane together.
+__device__ __forceinline__ int slot(int n) {
+    return (n & ~31) | ((n >> 2) & 3) << 3 | ((n >> 4) & 1) << 2 | (n & 3);
+}
+
+// x = out[0] + out[1] + ...
+template <int NP>
+__device__ __forceinline__ void split8(const float *x, bf16x8 *out) {
+    typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        u32x4v w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+            if (p + 1 < NP) {
+                r[2 * i] -= __uint_as_float(w[i] << 16);
+                r[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        }
+        out[p] = __builtin_bit_cast(bf16x8, w);
+    }
+}
+// Two accumulator tiles as an operand.
+template <int NP>
+__device__ __forceinline__ void split_tiles(f32x4 lo, f32x4 hi, bf16x8 *out) {
+    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    split8<NP>(x, out);
+}
+
+// acc + A B over the products of parts up to order max(NA, NB) - 1, the smallest first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const bf16x8 *a, const bf16x8 *b, f32x4 acc) {
+    constexpr int top = (NA > NB ? NA : NB) - 1;
+#pragma unroll
+    for (int o = top; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i <= o; ++i)
+            if (i < NA && o - i < NB) acc = mfma_bf16(a[i], b[o - i], acc);
+    return acc;
+}
+
+// The rows of a chunk's q, k or v (or dy): `live` tokens `stride` elements apart.
+// VEC: through a buffer resource that ends with the last of them, so that a
+// load past it gives zeros without a branch (loads behind branches wait for one
+// another); the host sees to it that a chunk's offsets fit 31 bits.  Else by
+// pointer, element by element.
+template <typename T, bool VEC>
+struct Rows {
+    rsrc_t r;
+    const T *p;
+    uint32_t step;      // bytes between tokens
+    size_t stride;
+    int live, width;
+    __device__ __forceinline__ Rows(const T *base, size_t st, int lv, int w)
+        : p(base), step(static_cast<uint32_t>(st * sizeof(T))), stride(st), live(lv < kC ? lv : kC), width(w) {
+        if constexpr (VEC) r = make_rsrc(base, live > 0 ? (live - 1) * step + w * sizeof(T) : 0u);
+    }
+};
+
+// Eight consecutive stored values of token t as loaded; zero from `live` and from
+// `width` on.
+template <typename T> struct Eight { u32x4 q; };
+template <> struct Eight<float> { u32x4 a, b; };
+
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T> load_eight(const Rows<T, VEC> &rows, int t, int n) {
+    Eight<T> e;
+    if constexpr (VEC) {
+        const uint32_t off = n < rows.width ? t * rows.step + n * sizeof(T) : 0x80000000u;
+        if constexpr (sizeof(T) == 4) {
+            e.a = bld16(rows.r, off);
+            e.b = bld16(rows.r, off + 16);
+        } else {
+            e.q = bld16(rows.r, off);
+        }
+    } else {
+        const T *row = rows.p + t * rows.stride;
+        uint32_t u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (t >= rows.live || n + i >= rows.width) continue;
+            if constexpr (sizeof(T) == 4)
+                u[i] = __float_as_uint(row[n + i]);
+            else
+                u[i >> 1] |= static_cast<uint32_t>(row[n + i].bits) << (16 * (i & 1));
+        }
+        if constexpr (sizeof(T) == 4) {
+            e.a = u32x4{u[0], u[1], u[2], u[3]};
+            e.b = u32x4{u[4], u[5], u[6], u[7]};
+        } else {
+            e.q = u32x4{u[0], u[1], u[2], u[3]};
+        }
+    }
+    return e;
+}
+// One stored value as loaded (its bits), and what it stands for.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint32_t load_one(const Rows<T, VEC> &rows, int t, int n) {
+    if constexpr (VEC) {
+        const uint32_t off = n < rows.width ? t * rows.step + n * sizeof(T) : 0x80000000u;
+        if constexpr (sizeof(T) == 4) return bld4(rows.r, off);
+        else return __builtin_amdgcn_raw_buffer_load_b16(rows.r, off, 0, 0);
+    } else {
+        if (t >= rows.live || n >= rows.width) return 0u;
+        if constexpr (sizeof(T) == 4) return __float_as_uint(rows.p[t * rows.stride + n]);
+        else return rows.p[t * rows.stride + n].bits;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(bits);
+    } else {
+        const T v{static_cast<uint16_t>(bits)};
+        return ldf(&v);
+    }
+}
+__device__ __forceinline__ void widen(const Eight<float> &r, float *f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = __uint_as_float(r.a[i]);
+        f[4 + i] = __uint_as_float(r.b[i]);
+    }
+}
+__device__ __forceinline__ void widen(const Eight<bf16_t> &r, float *f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(r.q[i] << 16);
+        f[2 * i + 1] = __uint_as_float(r.q[i] & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void widen(const Eight<f16_t> &r, float *f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.q[i])));
+        f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.q[i] >> 16)));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void to_parts(const Eight<T> &r, bf16x8 *out) {
+    if constexpr (sizeof(T) == 2 && Parts<T>::in == 1) {
+        out[0] = __builtin_bit_cast(bf16x8, r.q);
+    } else {
+        float f[8];
+        widen(r, f);
+        split8<Parts<T>::in>(f, out);
+    }
+}
+
+// ds_read_b64_tr_b16: see the lane layout at lds_read_tr16 in scan_common.hpp.
+__device__ __forceinline__ bf16x4 read_tr(const __bf16 *p) {
+    typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(p));
+}
+
+// Rows of a chunk in LDS: [part][token][slot], padded by 16 bytes a row so that
+// sixteen rows' 16-byte reads fall on different banks.
+template <int N> struct Tile {
+    static constexpr int pitch = N + 8;          // elements
+    static constexpr int size = kC * pitch;
+};
+// Operand rows 16 i + c, columns of k-step kk.
+template <int N>
+__device__ __forceinline__ bf16x8 tile_rows(const __bf16 *t, int i, int kk, int lane) {
+    return *reinterpret_cast<const bf16x8 *>(t + (16 * i + (lane & 15)) * Tile<N>::pitch + 32 * kk +
+                                             8 * (lane >> 4));
+}
+// The tile transposed: operand rows are columns 16 nt + c, k runs over the
+// tokens of k-step kk in the order of two accumulator tiles.
+template <int N>
+__device__ __forceinline__ bf16x8 tile_cols(const __bf16 *t, int nt, int kk, int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    const __bf16 *p = t + (32 * kk + 4 * g + (l >> 2)) * Tile<N>::pitch + 32 * (nt >> 1) + 8 * (l & 3) + 4 * (nt & 1);
+    const bf16x4 lo = read_tr(p), hi = read_tr(p + 16 * Tile<N>::pitch);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Block (i, kk) of a lower-triangular 64 x 64 operand (rows 16 i, columns 32 kk)
+// among its kTri stored ones: 0 .. 1, then 2 + 2 (i - 2) + kk.
+__device__ __forceinline__ constexpr int lower_block(int i, int kk) { return i < 2 ? i : 2 * (i - 1) + kk; }
+__device__ __forceinline__ constexpr int lower_steps(int i) { return i < 2 ? 1 : 2; }
+
+// What delta_prep leaves for a chunk of a head: row factors, then T and
+// scale (tril(Q K^T) . D) diag(beta) as operands, block by block, part by part,
+// sixteen bytes a lane.
+template <typename T> struct Record {
+    static constexpr int kK = 0, kQ = 64, kU = 128, kEnd = 192;    // floats: exp(G) rk, scale exp(G) rq,
+                                                                   // beta exp(G_C - G) rk, exp(G_C)
+    static constexpr size_t factors = 1024;
+    static constexpr size_t tri(int parts) { return size_t(kTri) * parts * 1024; }
+    static constexpr size_t t_at = factors, p_at = t_at + tri(kNP);
+    static constexpr size_t bytes = p_at + tri(Parts<T>::out);
+};
+
+}  // namespace delta
+}  // namespace m3

@@ -82,8 +82,9 @@ m3_status check_workspace(const m3_delta_inputs *in, size_t need) {
 extern "C" {
 
 size_t m3_delta_rule_workspace_bytes(const m3_delta_inputs *in) {
-    if (check(in) != M3_OK) return 0;
-    return 0;
+    if (check(in) != M3_OK || in->batch == 0) return 0;
+    const m3::DeltaLaunch a = launch_of(in);
+    return m3::delta_chunk_wanted(a) ? m3::delta_chunk_workspace(a) : 0;
 }
 
 m3_status m3_delta_rule(const m3_delta_inputs *in, void *y, float *state_out, void *stream) {
@@ -95,9 +96,18 @@ m3_status m3_delta_rule(const m3_delta_inputs *in, void *y, float *state_out, vo
     a.y = y;
     a.state_out = state_out;
     if (in->batch == 0) return m3::api_ok();
-    const hipError_t e = m3::launch_delta_recur(a, as_stream(stream));
+    int launches = 1;
+    hipError_t e;
+    if (m3::delta_chunk_wanted(a)) {
+        st = check_workspace(in, m3::delta_chunk_workspace(a));
+        if (st != M3_OK) return st;
+        launches = 0;
+        e = m3::launch_delta_chunk(a, in->workspace, as_stream(stream), launches);
+    } else {
+        e = m3::launch_delta_recur(a, as_stream(stream));
+    }
     if (e != hipSuccess) return m3::api_hip_fail(e, "delta rule launch");
-    m3::count_launches(1);
+    m3::count_launches(static_cast<uint64_t>(launches));
     return m3::api_ok();
 }
 
