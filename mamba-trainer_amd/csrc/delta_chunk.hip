@@ -184,35 +184,71 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
     emit(X, out + R::t_at, std::integral_constant<int, kNP>{});
 }
 
+// A chunk's operands in LDS.
+template <typename T, int N> struct Staged {
+    unsigned char k[Parts<T>::in][Tile<N>::bytes], q[Parts<T>::in][Tile<N>::bytes];
+    unsigned char v[sizeof(T) == 2 ? Tile<64>::bytes : 16];
+    unsigned char rec[Record<T>::bytes];
+};
+
 // One workgroup a (sequence, head, 64 columns of P), a wave 16 of them, the
-// chunks in turn; the next chunk's operands are on their way to registers while
-// this one's are multiplied.
+// chunks in turn.  bf16 with aligned rows: a chunk's operands go straight from
+// memory to LDS while the one before is multiplied (two buffers, one barrier a
+// chunk).  Other inputs become their bf16 parts on the way: through registers
+// into one buffer.
 template <typename T, int N, bool VEC>
-__global__ void __launch_bounds__(256) delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 32, NT = N / 16;
+    constexpr bool DMA = VEC && std::is_same<T, bf16_t>::value;
     using R = Record<T>;
     constexpr int pieces = kC * N / 8 / 256, rpieces = (R::bytes / 16 + 255) / 256;
-    __shared__ __attribute__((aligned(16))) __bf16 sk[KP * Tile<N>::size], sq[KP * Tile<N>::size];
-    __shared__ __attribute__((aligned(16))) unsigned char sr[R::bytes];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+    __shared__ __attribute__((aligned(1024))) Staged<T, N> staged[DMA ? 2 : 1];
+    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA ? 4 : 1][DMA ? kC : 1][16];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, kg = h / (a.heads / a.groups);
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
-    const int p = blockIdx.y * 64 + 16 * w + c;      // this lane's column
+    const int p0 = blockIdx.y * 64, p = p0 + 16 * w + c;      // this lane's column
     const T *kp = static_cast<const T *>(a.k) + b * L * a.ks + kg * n_of;
     const T *qp = static_cast<const T *>(a.q) + b * L * a.qs + kg * n_of;
     const T *vp = static_cast<const T *>(a.v) + b * L * a.vs + h * P;
-    T *yp = static_cast<T *>(a.y) + (b * L * a.heads + h) * P + p;
+    T *yp = static_cast<T *>(a.y) + (b * L * a.heads + h) * P;
     const size_t ystep = a.heads * P;
     f32x4 S[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = 16 * nt + 4 * g + r;
+            const int n = state_n(nt, g, r);
             S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
         }
     const int live = (len + kC - 1) / kC;
+    // the fetch of a chunk, in four parts; DMA: to LDS
+    const uint32_t dk = dma_at<T, N>(a.ks, n_of, 0, w, lane), dq = dma_at<T, N>(a.qs, n_of, 0, w, lane);
+    const uint32_t dv = dma_at<T, 64>(a.vs, P, p0, w, lane);
+    const auto dma = [&](int ck, int part) {
+        Staged<T, N> &to = staged[DMA ? ck & 1 : 0];
+        const size_t t0 = static_cast<size_t>(ck) * kC;
+        const int left = len - ck * kC;
+        if (part == 0) dma_tile<N>(Rows<T, true>(kp + t0 * a.ks, a.ks, left, n_of), dk, to.k[0], w);
+        if (part == 1) dma_tile<N>(Rows<T, true>(qp + t0 * a.qs, a.qs, left, n_of), dq, to.q[0], w);
+        if (part == 2) dma_tile<64>(Rows<T, true>(vp + t0 * a.vs, a.vs, left, P), dv, to.v, w);
+        if (part >= 2) {
+            const rsrc_t rec = make_rsrc(records + (bh * chunks + ck) * R::bytes, R::bytes);
+            constexpr int units = R::bytes / 1024, half = (units + 7) / 8;
+#pragma unroll
+            for (int i = 0; i < half; ++i) {
+                const int u = w + 4 * (i + (part - 2) * half);
+                if (u < units) scan::lds_dma16(rec, scan::lds_addr(to.rec + u * 1024), u * 1024 + lane * 16);
+            }
+        }
+    };
+    // else: to registers
+    const int kt0 = tid / (N / 8), kn = tid % (N / 8) * 8;
+    const uint32_t k_at = row_off<T>(a.ks, n_of, kt0, kn), q_at = row_off<T>(a.qs, n_of, kt0, kn);
+    const uint32_t v_at = row_off<T>(a.vs, P, 4 * g, p), y_at = row_off<T>(ystep, P, 4 * g, p);
     Eight<T> k8[pieces], q8[pieces];
     u32x4 r8[rpieces];
     uint32_t v[4][4];
@@ -223,9 +259,8 @@ __global__ void __launch_bounds__(256) delta_chunks(DeltaLaunch a, const unsigne
         const Rows<T, VEC> vr(vp + t0 * a.vs, a.vs, left, P);
 #pragma unroll
         for (int i = 0; i < pieces; ++i) {
-            const int id = tid + 256 * i, t = id / (N / 8), n = id % (N / 8) * 8;
-            k8[i] = load_eight(kr, t, n);
-            q8[i] = load_eight(qr, t, n);
+            k8[i] = load_eight(kr, k_at, kt0, kn, i * (2048 / N));
+            q8[i] = load_eight(qr, q_at, kt0, kn, i * (2048 / N));
         }
         const rsrc_t rec = make_rsrc(records + (bh * chunks + ck) * R::bytes, R::bytes);
 #pragma unroll
@@ -233,57 +268,105 @@ __global__ void __launch_bounds__(256) delta_chunks(DeltaLaunch a, const unsigne
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[i][r] = load_one(vr, 16 * i + 4 * g + r, p);
+            for (int r = 0; r < 4; ++r) v[i][r] = load_one(vr, v_at, 4 * g, p, 16 * i + r);
     };
-    if (live > 0) fetch(0);
-    for (int ck = 0; ck < live; ++ck) {
-        __syncthreads();
+    const auto put = [&]() {
 #pragma unroll
         for (int i = 0; i < pieces; ++i) {
-            const int id = tid + 256 * i, t = id / (N / 8), n = id % (N / 8) * 8;
             bf16x8 x[KP];
-            const auto put = [&](const Eight<T> &e, __bf16 *tile) {
-                to_parts(e, x);
+            const int at = tile_at<N>(kt0 + i * (2048 / N), kn / 8);
+            to_parts(k8[i], x);
 #pragma unroll
-                for (int q = 0; q < KP; ++q) {
-                    __bf16 *row = tile + q * Tile<N>::size + t * Tile<N>::pitch;
-                    *reinterpret_cast<bf16x4 *>(row + slot(n)) = __builtin_shufflevector(x[q], x[q], 0, 1, 2, 3);
-                    *reinterpret_cast<bf16x4 *>(row + slot(n + 4)) = __builtin_shufflevector(x[q], x[q], 4, 5, 6, 7);
-                }
-            };
-            put(k8[i], sk);
-            put(q8[i], sq);
+            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(staged[0].k[q] + at) = x[q];
+            to_parts(q8[i], x);
+#pragma unroll
+            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(staged[0].q[q] + at) = x[q];
         }
 #pragma unroll
         for (int i = 0; i < rpieces; ++i)
-            if (tid + 256 * i < static_cast<int>(R::bytes / 16)) reinterpret_cast<u32x4 *>(sr)[tid + 256 * i] = r8[i];
+            if (tid + 256 * i < static_cast<int>(R::bytes / 16))
+                reinterpret_cast<u32x4 *>(staged[0].rec)[tid + 256 * i] = r8[i];
+    };
+    if (live > 0) {
+        if constexpr (DMA) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dma(0, i);
+        } else {
+            fetch(0);
+        }
+    }
+    for (int ck = 0; ck < live; ++ck) {
+        const Staged<T, N> &st = staged[DMA ? ck & 1 : 0];
         f32x4 e[4];
+        if constexpr (DMA) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        } else {
+            __syncthreads();
+            put();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) e[i][r] = value_of<T>(v[i][r]);
-        __syncthreads();
-        if (ck + 1 < live) fetch(ck + 1);
-        const float *fac = reinterpret_cast<const float *>(sr);
-        f32x4 y[4];
-        // R and the state's part of Y
+                for (int r = 0; r < 4; ++r) e[i][r] = value_of<T>(v[i][r]);
+            __syncthreads();
+            if (ck + 1 < live) fetch(ck + 1);
+        }
+        const float *fac = reinterpret_cast<const float *>(st.rec);
+        // R and the state's part of Y: while a k-step is multiplied, the next one's
+        // operands are read and its columns of S are split
+        f32x4 y[4], ks[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 ks[4] = {y[0], y[0], y[0], y[0]};
+        for (int i = 0; i < 4; ++i) y[i] = ks[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        bf16x8 kf[2][4][KP], qf[2][4][KP], sp[2][kNP];
+        const auto rows = [&](int kk) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < KP; ++q) {
+                    kf[kk & 1][i][q] = tile_rows<N>(st.k[q], i, kk, lane);
+                    qf[kk & 1][i][q] = tile_rows<N>(st.q[q], i, kk, lane);
+                }
+        };
+        // blocks of a triangle: those of the first k-step, then the second's
+        constexpr int at4[4] = {0, 1, 2, 4}, at2[2] = {3, 5};
+        const auto tri = [&](size_t at, int np, int blk, int q) {
+            return *reinterpret_cast<const bf16x8 *>(st.rec + at + ((blk * np + q) * 64 + lane) * 16);
+        };
+        bf16x8 t4[4][kNP], t2[2][kNP];
+        rows(0);
+        split_tiles<kNP>(S[0], S[1], sp[0]);
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
-            bf16x8 s[kNP];
-            split_tiles<kNP>(S[2 * kk], S[2 * kk + 1], s);
+            if (kk + 1 < KS) {
+                rows(kk + 1);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bf16x8 x[KP];
+                for (int q = 0; q < kNP; ++q) {
 #pragma unroll
-                for (int q = 0; q < KP; ++q) x[q] = tile_rows<N>(sk + q * Tile<N>::size, i, kk, lane);
-                ks[i] = mma_parts<KP, kNP>(x, s, ks[i]);
+                    for (int i = 0; i < 4; ++i) t4[i][q] = tri(R::t_at, kNP, at4[i], q);
 #pragma unroll
-                for (int q = 0; q < KP; ++q) x[q] = tile_rows<N>(sq + q * Tile<N>::size, i, kk, lane);
-                y[i] = mma_parts<KP, YP>(x, s, y[i]);
+                    for (int i = 0; i < 2; ++i) t2[i][q] = tri(R::t_at, kNP, at2[i], q);
+                }
+                if constexpr (DMA) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bf16x4 x = tile_acc(st.v, i, w, lane);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) e[i][r] = static_cast<float>(x[r]);
+                    }
+                }
             }
+            if constexpr (DMA) {
+                if (ck + 1 < live)
+#pragma unroll
+                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) dma(ck + 1, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
+            mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
+            mma_rows<4, KP, YP>(qf[kk & 1], sp[kk & 1], y);
+            interleave<4 * (3 + 2), 3>();
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -293,67 +376,81 @@ __global__ void __launch_bounds__(256) delta_chunks(DeltaLaunch a, const unsigne
             y[i] *= fq;
         }
         // E = T R
-        const auto tri = [&](size_t at, int np, int blk, int q) {
-            return *reinterpret_cast<const bf16x8 *>(sr + at + ((blk * np + q) * 64 + lane) * 16);
-        };
         bf16x8 x[2][kNP];
         split_tiles<kNP>(e[0], e[1], x[0]);
         split_tiles<kNP>(e[2], e[3], x[1]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            e[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) e[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        mma_rows<4, kNP, kNP>(t4, x[0], e);
+        mma_rows<2, kNP, kNP>(t2, x[1], e + 2);
+        // S, and Y's part within the chunk
+        bf16x8 p4[4][YP], p2[2][YP], xe[2][YP];
+        bf16x8 kt[2][4][KP];    // four tiles of N at one k-step
+        const auto cols = [&](int j) {
 #pragma unroll
-            for (int kk = 0; kk < lower_steps(i); ++kk) {
-                bf16x8 t[kNP];
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int q = 0; q < kNP; ++q) t[q] = tri(R::t_at, kNP, lower_block(i, kk), q);
-                e[i] = mma_parts<kNP, kNP>(t, x[kk], e[i]);
-            }
-        }
-        // Y
-        split_tiles<YP>(e[0], e[1], x[0]);
-        split_tiles<YP>(e[2], e[3], x[1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int kk = 0; kk < lower_steps(i); ++kk) {
-                bf16x8 t[YP];
-#pragma unroll
-                for (int q = 0; q < YP; ++q) t[q] = tri(R::p_at, YP, lower_block(i, kk), q);
-                y[i] = mma_parts<YP, YP>(t, x[kk], y[i]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = ck * kC + 16 * i + 4 * g + r;
-                if (t < len && p < P) stf(yp + t * ystep, y[i][r]);
-            }
-        }
-        // S
+                for (int q = 0; q < KP; ++q)
+                    kt[j & 1][i][q] = tile_cols<N>(st.k[q], 4 * (j >> 1) + i, j & 1, lane);
+        };
+        cols(0);
+        split_tiles<YP>(e[0], e[1], xe[0]);
+        split_tiles<YP>(e[2], e[3], xe[1]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] *= *reinterpret_cast<const f32x4 *>(fac + R::kU + 16 * i + 4 * g);
         split_tiles<kNP>(e[0], e[1], x[0]);
         split_tiles<kNP>(e[2], e[3], x[1]);
         const float end = fac[R::kEnd];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            S[nt] *= end;
+        for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                bf16x8 kt[KP];
+        for (int j = 0; j < NT / 2; ++j) {
+            if (j + 1 < NT / 2) {
+                cols(j + 1);
+            } else {
 #pragma unroll
-                for (int q = 0; q < KP; ++q) kt[q] = tile_cols<N>(sk + q * Tile<N>::size, nt, kk, lane);
-                S[nt] = mma_parts<KP, kNP>(kt, x[kk], S[nt]);
+                for (int q = 0; q < YP; ++q) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p4[i][q] = tri(R::p_at, YP, at4[i], q);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) p2[i][q] = tri(R::p_at, YP, at2[i], q);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            mma_rows<4, KP, kNP>(kt[j & 1], x[j & 1], S + 4 * (j >> 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mma_rows<4, YP, YP>(p4, xe[0], y);
+        mma_rows<2, YP, YP>(p2, xe[1], y + 2);
+        // padding rows past the buffer's end are dropped
+        const Rows<T, VEC> yr(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
+        if constexpr (DMA) {
+            // the wave's 16 columns through LDS to 16-byte stores
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    sy[w][16 * i + 4 * g + r][c] = from_f32<bf16_t>(y[i][r]).bits;
+            const uint32_t at = row_off<T>(ystep, P, lane >> 1, p0 + 16 * w + 8 * (lane & 1));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                bst16(*reinterpret_cast<const u32x4 *>(&sy[w][32 * i + (lane >> 1)][8 * (lane & 1)]), yr.r,
+                      at + 32 * i * yr.step);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) store_one(yr, y_at, 4 * g, p, 16 * i + r, y[i][r]);
         }
     }
     if (p >= P) return;
-    for (int t = len + g; t < L; t += 4) stf(yp + t * ystep, 0.f);
+    for (int t = len + g; t < L; t += 4) stf(yp + t * ystep + p, 0.f);
     if (a.state_out == nullptr) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = 16 * nt + 4 * g + r;
+            const int n = state_n(nt, g, r);
             if (n < n_of) a.state_out[(bh * P + p) * n_of + n] = S[nt][r];
         }
 }
@@ -364,12 +461,15 @@ hipError_t by_state(size_t d_state, F f) {
     return f(std::integral_constant<int, 128>{});
 }
 
-// 16-byte loads of q and k rows: whole pieces of eight, every row aligned; a
-// chunk's offsets below 2^31.
-bool qk_vec(const DeltaLaunch &a, size_t size) {
-    const size_t most = (size_t(1) << 31) / (kC * size) - 1024;
-    return a.d_state % 8 == 0 && a.qs < most && a.ks < most && a.vs < most && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 &&
-           (reinterpret_cast<uintptr_t>(a.k) & 15) == 0 && a.qs * size % 16 == 0 && a.ks * size % 16 == 0;
+// 16-byte access to the rows of q, k, v and y: whole pieces of eight, every row
+// aligned; a chunk's offsets below 2^31.
+bool rows_vec(const DeltaLaunch &a, size_t size) {
+    const auto ok = [&](const void *p, size_t stride) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0 &&
+               (stride + 1024) * size * kC < size_t(1) << 31;
+    };
+    return a.d_state % 8 == 0 && a.head_dim % 8 == 0 && ok(a.q, a.qs) && ok(a.k, a.ks) && ok(a.v, a.vs) &&
+           ok(a.y, a.heads * a.head_dim);
 }
 
 size_t chunks_of(const DeltaLaunch &a) { return (a.seq + kC - 1) / kC; }
@@ -403,7 +503,7 @@ hipError_t launch_delta_chunk(const DeltaLaunch &a, void *workspace, hipStream_t
                 launches += 2;
                 return hipGetLastError();
             };
-            return qk_vec(a, sizeof(T)) ? go(std::true_type{}) : go(std::false_type{});
+            return rows_vec(a, sizeof(T)) ? go(std::true_type{}) : go(std::false_type{});
         });
     });
 }

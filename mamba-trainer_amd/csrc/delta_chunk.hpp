@@ -23,10 +23,13 @@
 // two accumulator tiles (rows 4g .. 4g+3 of each) are an operand as they lie.
 // So a wave that owns 16 columns of P takes its columns of S, R and E from
 // product to product in registers; what it reads from LDS are the chunk's own
-// operands, stored in that order (`slot`).
+// operands.  Rows of S's tiles are n = 32 (nt / 2) + 8g + 4 (nt % 2) + r, so that
+// the pair of them takes eight consecutive n of a K row; rows of R's and E's
+// tiles are tokens 16 i + 4g + r.
 #pragma once
 
 #include "delta.hpp"
+#include "scan_common.hpp"
 
 namespace m3 {
 namespace delta {
@@ -40,11 +43,6 @@ template <> struct Parts<bf16_t> { static constexpr int in = 1, out = 2; };
 template <> struct Parts<f16_t> { static constexpr int in = 2, out = 2; };
 template <> struct Parts<float> { static constexpr int in = 3, out = 3; };
 constexpr int kNP = 3;          // of an f32 value on the way of the state
-
-// Where column n of a row lies in LDS: the eight k-slots of a lane together.
-__device__ __forceinline__ int slot(int n) {
-    return (n & ~31) | ((n >> 2) & 3) << 3 | ((n >> 4) & 1) << 2 | (n & 3);
-}
 
 // x = out[0] + out[1] + ...
 template <int NP>
@@ -74,16 +72,34 @@ __device__ __forceinline__ void split_tiles(f32x4 lo, f32x4 hi, bf16x8 *out) {
     split8<NP>(x, out);
 }
 
-// acc + A B over the products of parts up to order max(NA, NB) - 1, the smallest first.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mma_parts(const bf16x8 *a, const bf16x8 *b, f32x4 acc) {
+// acc[m] + A[m] B for M tiles over the products of parts up to order max(NA, NB)
+// - 1, the smallest first.  The tiles take turns, so that no product waits for
+// the one before it.
+template <int M, int NA, int NB>
+__device__ __forceinline__ void mma_rows(const bf16x8 (*a)[NA], const bf16x8 *b, f32x4 *acc) {
     constexpr int top = (NA > NB ? NA : NB) - 1;
 #pragma unroll
     for (int o = top; o >= 0; --o)
 #pragma unroll
         for (int i = 0; i <= o; ++i)
-            if (i < NA && o - i < NB) acc = mfma_bf16(a[i], b[o - i], acc);
+            if (i < NA && o - i < NB)
+#pragma unroll
+                for (int m = 0; m < M; ++m) acc[m] = mfma_bf16(a[m][i], b[o - i], acc[m]);
+}
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const bf16x8 *a, const bf16x8 *b, f32x4 acc) {
+    mma_rows<1, NA, NB>(reinterpret_cast<const bf16x8(*)[NA]>(a), b, &acc);
     return acc;
+}
+// Matrix products of a region in turn with the vector work beside them: `n`
+// times one MFMA and `valu` VALU instructions.
+template <int n, int valu>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, valu, 0);
+    }
 }
 
 // The rows of a chunk's q, k or v (or dy): `live` tokens `stride` elements apart.
@@ -104,28 +120,36 @@ struct Rows {
     }
 };
 
-// Eight consecutive stored values of token t as loaded; zero from `live` and from
+// Byte offset of values n, n + 1, .. of token t in such rows, past any range from
 // `width` on.
+template <typename T>
+__device__ __forceinline__ uint32_t row_off(size_t stride, int width, int t, int n) {
+    return n < width ? (t * static_cast<uint32_t>(stride) + n) * static_cast<uint32_t>(sizeof(T)) : 0x80000000u;
+}
+
+// Eight consecutive stored values of token t + dt as loaded; zero from `live` and
+// from `width` on.  VEC reads at off + dt * step, off = row_off(t, n): what does
+// not change from chunk to chunk stays with the caller.
 template <typename T> struct Eight { u32x4 q; };
 template <> struct Eight<float> { u32x4 a, b; };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ Eight<T> load_eight(const Rows<T, VEC> &rows, int t, int n) {
+__device__ __forceinline__ Eight<T> load_eight(const Rows<T, VEC> &rows, uint32_t off, int t, int n, int dt) {
     Eight<T> e;
     if constexpr (VEC) {
-        const uint32_t off = n < rows.width ? t * rows.step + n * sizeof(T) : 0x80000000u;
+        const uint32_t o = off + dt * rows.step;
         if constexpr (sizeof(T) == 4) {
-            e.a = bld16(rows.r, off);
-            e.b = bld16(rows.r, off + 16);
+            e.a = bld16(rows.r, o);
+            e.b = bld16(rows.r, o + 16);
         } else {
-            e.q = bld16(rows.r, off);
+            e.q = bld16(rows.r, o);
         }
     } else {
-        const T *row = rows.p + t * rows.stride;
+        const T *row = rows.p + (t + dt) * rows.stride;
         uint32_t u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (t >= rows.live || n + i >= rows.width) continue;
+            if (t + dt >= rows.live || n + i >= rows.width) continue;
             if constexpr (sizeof(T) == 4)
                 u[i] = __float_as_uint(row[n + i]);
             else
@@ -140,17 +164,34 @@ __device__ __forceinline__ Eight<T> load_eight(const Rows<T, VEC> &rows, int t, 
     }
     return e;
 }
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T> load_eight(const Rows<T, VEC> &rows, int t, int n) {
+    return load_eight(rows, row_off<T>(rows.stride, rows.width, t, n), t, n, 0);
+}
 // One stored value as loaded (its bits), and what it stands for.
 template <typename T, bool VEC>
-__device__ __forceinline__ uint32_t load_one(const Rows<T, VEC> &rows, int t, int n) {
+__device__ __forceinline__ uint32_t load_one(const Rows<T, VEC> &rows, uint32_t off, int t, int n, int dt) {
     if constexpr (VEC) {
-        const uint32_t off = n < rows.width ? t * rows.step + n * sizeof(T) : 0x80000000u;
-        if constexpr (sizeof(T) == 4) return bld4(rows.r, off);
-        else return __builtin_amdgcn_raw_buffer_load_b16(rows.r, off, 0, 0);
+        const uint32_t o = off + dt * rows.step;
+        if constexpr (sizeof(T) == 4) return bld4(rows.r, o);
+        else return __builtin_amdgcn_raw_buffer_load_b16(rows.r, o, 0, 0);
     } else {
-        if (t >= rows.live || n >= rows.width) return 0u;
-        if constexpr (sizeof(T) == 4) return __float_as_uint(rows.p[t * rows.stride + n]);
-        else return rows.p[t * rows.stride + n].bits;
+        if (t + dt >= rows.live || n >= rows.width) return 0u;
+        if constexpr (sizeof(T) == 4) return __float_as_uint(rows.p[(t + dt) * rows.stride + n]);
+        else return rows.p[(t + dt) * rows.stride + n].bits;
+    }
+}
+// The same rows written: a value past their range is dropped.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_one(const Rows<T, VEC> &rows, uint32_t off, int t, int n, int dt, float v) {
+    T x;
+    stf(&x, v);
+    if constexpr (VEC) {
+        const uint32_t o = off + dt * rows.step;
+        if constexpr (sizeof(T) == 4) bst4(__float_as_uint(x), rows.r, o);
+        else bst2(x.bits, rows.r, o);
+    } else {
+        if (t + dt < rows.live && n < rows.width) const_cast<T *>(rows.p)[(t + dt) * rows.stride + n] = x;
     }
 }
 template <typename T>
@@ -194,32 +235,60 @@ __device__ __forceinline__ void to_parts(const Eight<T> &r, bf16x8 *out) {
     }
 }
 
-// ds_read_b64_tr_b16: see the lane layout at lds_read_tr16 in scan_common.hpp.
-__device__ __forceinline__ bf16x4 read_tr(const __bf16 *p) {
-    typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(p));
+// Rows of a chunk in LDS, [token][N] of 16-bit values, a row's 16-byte pieces
+// permuted so that both ways of reading them fall on different banks: sixteen
+// rows' pieces at one place (an operand's rows), and four rows' by four pieces
+// (a transposed operand).
+template <int N>
+__device__ __forceinline__ constexpr int swizzle(int t) {
+    return N == 128 ? (t & 3) << 2 | ((t >> 2) & 3) : ((t >> 1) & 1) << 2 | ((t >> 2) & 3);
+}
+template <int N> struct Tile {
+    static constexpr int bytes = kC * N * 2;
+};
+template <int N>
+__device__ __forceinline__ int tile_at(int t, int piece) {
+    return t * (2 * N) + ((piece ^ swizzle<N>(t)) << 4);
+}
+// Operand rows 16 i + c, columns 32 kk + 8g ..
+template <int N>
+__device__ __forceinline__ bf16x8 tile_rows(const unsigned char *t, int i, int kk, int lane) {
+    return *reinterpret_cast<const bf16x8 *>(t + 16 * i * (2 * N) + tile_at<N>(lane & 15, 4 * kk + (lane >> 4)));
+}
+// The tile transposed: operand rows are the n of tile nt, k runs over the tokens
+// of k-step kk in the order of two accumulator tiles.
+template <int N>
+__device__ __forceinline__ bf16x8 tile_cols(const unsigned char *t, int nt, int kk, int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    const unsigned char *p = t + 32 * kk * (2 * N) + tile_at<N>(4 * g + (l >> 2), 4 * (nt >> 1) + (l & 3)) + 8 * (nt & 1);
+    const bf16x4 lo = scan::lds_read_tr16(reinterpret_cast<const __bf16 *>(p));
+    const bf16x4 hi = scan::lds_read_tr16(reinterpret_cast<const __bf16 *>(p + 16 * (2 * N)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Sixteen columns from 16 w on of a 64-wide tile as accumulator tile i holds them.
+__device__ __forceinline__ bf16x4 tile_acc(const unsigned char *t, int i, int w, int lane) {
+    const int l = lane & 15, g = lane >> 4, q = l & 3;
+    const unsigned char *p = t + 16 * i * 128 + tile_at<64>(4 * g + (l >> 2), 2 * w + (q >> 1)) + 8 * (q & 1);
+    return scan::lds_read_tr16(reinterpret_cast<const __bf16 *>(p));
+}
+// The n of row r of lane group g of S's tile nt.
+__device__ __forceinline__ constexpr int state_n(int nt, int g, int r) {
+    return 32 * (nt >> 1) + 8 * g + 4 * (nt & 1) + r;
 }
 
-// Rows of a chunk in LDS: [part][token][slot], padded by 16 bytes a row so that
-// sixteen rows' 16-byte reads fall on different banks.
-template <int N> struct Tile {
-    static constexpr int pitch = N + 8;          // elements
-    static constexpr int size = kC * pitch;
-};
-// Operand rows 16 i + c, columns of k-step kk.
-template <int N>
-__device__ __forceinline__ bf16x8 tile_rows(const __bf16 *t, int i, int kk, int lane) {
-    return *reinterpret_cast<const bf16x8 *>(t + (16 * i + (lane & 15)) * Tile<N>::pitch + 32 * kk +
-                                             8 * (lane >> 4));
+// A tile's rows straight from memory to LDS by one of four waves: kilobytes w, w
+// + 4, ..  `at` is this lane's place (dma_at), the same for all of them.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t dma_at(size_t stride, int width, int n0, int w, int lane) {
+    const int t = w * (512 / N) + lane / (N / 8);
+    const int n = n0 + ((lane % (N / 8)) ^ swizzle<N>(t)) * 8;
+    return row_off<T>(stride, width, t, n);
 }
-// The tile transposed: operand rows are columns 16 nt + c, k runs over the
-// tokens of k-step kk in the order of two accumulator tiles.
-template <int N>
-__device__ __forceinline__ bf16x8 tile_cols(const __bf16 *t, int nt, int kk, int lane) {
-    const int l = lane & 15, g = lane >> 4;
-    const __bf16 *p = t + (32 * kk + 4 * g + (l >> 2)) * Tile<N>::pitch + 32 * (nt >> 1) + 8 * (l & 3) + 4 * (nt & 1);
-    const bf16x4 lo = read_tr(p), hi = read_tr(p + 16 * Tile<N>::pitch);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+template <int N, typename R>
+__device__ __forceinline__ void dma_tile(const R &rows, uint32_t at, unsigned char *tile, int w) {
+#pragma unroll
+    for (int i = 0; i < N / 32; ++i)
+        scan::lds_dma16(rows.r, scan::lds_addr(tile + (w + 4 * i) * 1024), at + i * (2048 / N) * rows.step);
 }
 
 // Block (i, kk) of a lower-triangular 64 x 64 operand (rows 16 i, columns 32 kk)
