@@ -69,7 +69,7 @@ m3_status m3_delta_step(const m3_delta_inputs *in, float *state, void *y, void *
  * the window, or NULL) are given; dq, dk [B, T, G, N], dv [B, T, H, P] in the
  * inputs' type, dg, dbeta [B, T, H] and dstate0 [B, H, P, N] (NULL without
  * in->state) are written, all contiguous.  dq and dk are summed over the heads
- * that share a group. */
+ * that share a group.  d_state up to 128, else M3_ERR_UNSUPPORTED. */
 typedef struct m3_delta_grads {
     const void *dy;
     const float *dstate;

@@ -40,6 +40,8 @@ bool delta_chunk_wanted(const DeltaLaunch &a);
 size_t delta_chunk_workspace(const DeltaLaunch &a);
 hipError_t launch_delta_chunk(const DeltaLaunch &a, void *workspace, hipStream_t s, int &launches);
 
+// Gradients (delta_backward.hip): the shapes covered, the workspace, the launch.
+bool delta_backward_supported(const DeltaLaunch &a);
 size_t delta_backward_workspace(const DeltaLaunch &a);
 hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void *workspace,
                                  hipStream_t s, int &launches);

@@ -1,210 +1,597 @@
-// Gradients of the gated delta rule on gfx950, by the reverse of its
-// recurrence (S~ = exp(g) S, e = v - S~ k, u = beta e, S' = S~ + u k^T,
-// y = scale S' q):
-//   dS' += scale dy q^T;  dq = scale S'^T dy;  du = dS' k;  dk = dS'^T u
-//   dbeta = du . e;  de = beta du;  dv = de
-//   dS~ = dS' - de k^T;  dk -= S~^T de;  dg = <dS~, S~>;  dS = exp(g) dS~
-// Two launches a sequence walk: forward, leaving every S~ in the workspace,
-// and back; a third sums dq and dk over the heads of a group and takes them
-// through the unit-length norm.
-#include "delta.hpp"
+// Gradients of the gated delta rule, chunk by chunk on the MFMA (gfx950); the
+// chunk's notation, numbers and layouts are in delta_chunk.hpp.
+//
+// Given dY and the gradient dS1 of the state after a chunk, with P the attention
+// scale (tril(Q K^T) . D), row factors fQ = scale exp(G) rq, fK = exp(G) rk and
+// fU = beta exp(G_C - G) rk on raw rows q, k:
+//   dR = T^T ((P diag(beta))^T dY + diag(fU) K dS1^T);  dV = dR
+//   dS0 = exp(G_C) dS1 + (diag(fQ) dY)^T Q - (diag(fK) dR)^T K
+// passes from the last chunk to the first, column by column of P as the forward
+// does (delta_reverse).  The rest is each chunk's own (delta_grads): with F = dY
+// E^T and Z = dR E^T,
+//   X_ij = scale rq_i rk_j D_ij beta_j F_ij (j <= i),  Y_ij = rk_i rk_j D_ij beta_j Z_ij (j < i)
+//   rq dq^ = diag(fQ) dY S0 + X K
+//   rk dk^ = diag(fU) E dS1 - diag(fK) dR S0 + X^T Q - (Y + Y^T) K
+//   V_ij = X_ij / beta_j (q_i.k_j) - Y_ij / beta_j (k_i.k_j)
+//   dbeta_j = sum_i V_ij + (fU_j / beta_j) k_j.(E dS1)_j
+//   dg_t = sum_{j<t<=i} beta_j V_ij + sum_{i>=t} a_i + sum_{j<t} b_j + exp(G_C) <dS1, S0>
+//     a_i = fQ_i q_i.(dY S0)_i - fK_i k_i.(dR S0)_i,  b_j = fU_j k_j.(E dS1)_j
+// (nothing is divided by beta), and through the unit-length norm dq = rq dq^ - q
+// rq^2 (q . rq dq^), dk alike.  The first sum of dg_t is over a rectangle of the
+// triangle: as the suffix sum of row sums less column sums, in f64, where the
+// entries outside the rectangle cancel exactly.
+#include "delta_chunk.hpp"
 
 namespace m3 {
 namespace {
 
 using namespace delta;
 
-constexpr int kThreads = 256;
-
-__device__ float block_sum(float v, float *red) {
-    v = group_sum(v, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < kThreads / 64; ++i) s += red[i];
-    return s;
-}
-
-// One workgroup a (sequence, head): thread i holds rows of P through LDS
-// vectors of k and q; S lives in global memory (states).
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-delta_backward_walk(DeltaLaunch a, DeltaGrads gr, float *states, float *dqh, float *dkh, float *dS) {
-    extern __shared__ float lds[];
-    __shared__ float red[kThreads / 64];
-    const int tid = threadIdx.x;
-    const int N = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim), PN = P * N;
-    float *kv = lds, *qv = kv + N, *ev = qv + N, *uv = ev + P, *yv = uv + P;
-    const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, kg = h / (a.heads / a.groups);
+// One workgroup a (sequence, head, 64 columns of P), a wave 16 of them, the
+// chunks from the last to the first.
+template <typename T, int N, bool VEC>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chunks, float *kept) {
+    constexpr int KP = Parts<T>::in, KS = N / 32, NT = N / 16;
+    using St = Stage<T, N, VEC, true, 1 + 2 * kTriT, kTriT>;
+    constexpr bool DMA = St::DMA;
+    constexpr size_t rec_bytes = BackRecord::units * 1024;
+    __shared__ __attribute__((aligned(1024))) typename St::Buf staged[DMA ? 2 : 1];
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
-    float *st = states + bh * L * PN;
-    float *ds = dS + bh * PN;
-    const auto load_kq = [&](size_t tok) {
-        __syncthreads();
-        const T *kp = static_cast<const T *>(a.k) + tok * a.ks + kg * N;
-        const T *qp = static_cast<const T *>(a.q) + tok * a.qs + kg * N;
-        float sk = 0.f, sq = 0.f;
-        for (int i = tid; i < N; i += kThreads) {
-            const float x = ldf(kp + i), y = ldf(qp + i);
-            kv[i] = x;
-            qv[i] = y;
-            sk += x * x;
-            sq += y * y;
+    const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
+    const int p0 = blockIdx.y * 64, p = p0 + 16 * w + c;      // this lane's column
+    const size_t pv = a.heads * P, row0 = (b * L * a.heads + h) * P;
+    T *dvp = static_cast<T *>(gr.dv) + row0;
+    const uint32_t dv_at = row_off<T>(pv, P, 4 * g, p);
+    const Kept kd(a);
+    f32x4 S[NT];   // the gradient of the state after the chunk
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = state_n(nt, g, r);
+            S[nt][r] = gr.dstate && p < P && n < n_of ? gr.dstate[(bh * P + p) * n_of + n] : 0.f;
         }
-        if (a.qk_norm) {
-            const float rk = 1.0f / sqrtf(block_sum(sk, red) + kUnitEps);
-            const float rq = 1.0f / sqrtf(block_sum(sq, red) + kUnitEps);
-            for (int i = tid; i < N; i += kThreads) {
-                kv[i] *= rk;
-                qv[i] *= rq;
-            }
-        }
-        __syncthreads();
-    };
-    // forward: st[t] = S~ of token t
-    for (int t = 0; t < len; ++t) {
-        const size_t tok = b * L + t;
-        const float al = expf(clamp_decay(a.g[tok * a.heads + h]));
-        float *cur = st + static_cast<size_t>(t) * PN;
-        if (t > 0) {
-            const float *pre = cur - PN;
-            for (int i = tid; i < PN; i += kThreads) cur[i] = al * (pre[i] + uv[i / N] * kv[i % N]);
+    const int live = (len + kC - 1) / kC;
+    St in(a, b, h, len, static_cast<const T *>(gr.dy) + row0, pv, p0, records + bh * chunks * rec_bytes, rec_bytes);
+    if (live > 0) {
+        if constexpr (DMA) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) in.dma(staged[(live - 1) & 1], live - 1, i);
         } else {
-            for (int i = tid; i < PN; i += kThreads) cur[i] = a.state ? al * a.state[bh * PN + i] : 0.f;
+            in.fetch(live - 1);
         }
-        load_kq(tok);
-        const float beta = a.beta[tok * a.heads + h];
-        for (int p = tid; p < P; p += kThreads) {
-            float d = 0.f;
-            for (int i = 0; i < N; ++i) d += cur[p * N + i] * kv[i];
-            uv[p] = beta * (ldf(static_cast<const T *>(a.v) + tok * a.vs + h * P + p) - d);
-        }
-        __syncthreads();
     }
-    for (int i = tid; i < PN; i += kThreads) ds[i] = gr.dstate ? gr.dstate[bh * PN + i] : 0.f;
-    for (int t = L - 1; t >= len; --t) {
-        const size_t tok = b * L + t;
-        for (int i = tid; i < N; i += kThreads)
-            dqh[(tok * a.heads + h) * N + i] = dkh[(tok * a.heads + h) * N + i] = 0.f;
-        for (int p = tid; p < P; p += kThreads) stf(static_cast<T *>(gr.dv) + (tok * a.heads + h) * P + p, 0.f);
-        if (tid == 0) gr.dg[tok * a.heads + h] = gr.dbeta[tok * a.heads + h] = 0.f;
+    for (int ck = live - 1; ck >= 0; --ck) {
+        typename St::Buf &st = staged[DMA ? ck & 1 : 0], &next = staged[DMA ? (ck + 1) & 1 : 0];
+        f32x4 dy[4];
+        if constexpr (DMA) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        } else {
+            __syncthreads();
+            in.put(st);
+            in.values(st, dy);
+            __syncthreads();
+            if (ck > 0) in.fetch(ck - 1);
+        }
+        float *keep = kept + (bh * chunks + ck) * kd.floats();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<f32x4 *>(keep + kd.s1() + p * N + state_n(nt, g, 0)) = S[nt];
+        const float *fac = reinterpret_cast<const float *>(st.rec);
+        f32x4 ks[4], x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ks[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        bf16x8 kf[2][4][KP], sp[2][kNP], t4[4][kNP], t2[2][kNP], p4[4][kNP], p2[2][kNP];
+        const auto rows = [&](int kk) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < KP; ++q) kf[kk & 1][i][q] = tile_rows<N>(st.k[q], i, kk, lane);
+        };
+        rows(0);
+        split_tiles<kNP>(S[0], S[1], sp[0]);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            if (kk + 1 < KS) {
+                rows(kk + 1);
+            } else {
+                tri_load<kNP>(st.rec + (1 + kTriT) * 1024, lane, p4, p2, true);
+                if constexpr (DMA) in.values(st, dy);
+            }
+            if constexpr (DMA) {
+                if (ck > 0)
+#pragma unroll
+                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) in.dma(next, ck - 1, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
+            mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
+            interleave<4 * 3, 5>();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        tri_load<kNP>(st.rec + 1024, lane, t4, t2, true);
+        {
+            bf16x8 d[2][KP];
+            split_tiles<KP>(dy[0], dy[1], d[0]);
+            split_tiles<KP>(dy[2], dy[3], d[1]);
+            mma_rows<2, kNP, KP>(p2, d[0], x);
+            mma_rows<4, kNP, KP>(p4, d[1], x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += *reinterpret_cast<const f32x4 *>(fac + kFacU + 16 * i + 4 * g) * ks[i];
+        bf16x8 xs[2][kNP], ys[2][kNP];
+        split_tiles<kNP>(x[0], x[1], xs[0]);
+        split_tiles<kNP>(x[2], x[3], xs[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        mma_rows<2, kNP, kNP>(t2, xs[0], x);
+        mma_rows<4, kNP, kNP>(t4, xs[1], x);
+        // x is dR
+        const Rows<T, VEC> dvr(dvp + static_cast<size_t>(ck) * kC * pv, pv, len - ck * kC, P);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                keep[kd.dr() + (16 * i + 4 * g + r) * kd.p64 + p] = x[i][r];
+                store_one(dvr, dv_at, 4 * g, p, 16 * i + r, x[i][r]);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] *= -*reinterpret_cast<const f32x4 *>(fac + kFacK + 16 * i + 4 * g);
+            dy[i] *= *reinterpret_cast<const f32x4 *>(fac + kFacQ + 16 * i + 4 * g);
+        }
+        split_tiles<kNP>(x[0], x[1], xs[0]);
+        split_tiles<kNP>(x[2], x[3], xs[1]);
+        split_tiles<kNP>(dy[0], dy[1], ys[0]);
+        split_tiles<kNP>(dy[2], dy[3], ys[1]);
+        bf16x8 kt[2][4][KP], qt[2][4][KP];
+        const auto cols = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < KP; ++q) {
+                    kt[j & 1][i][q] = tile_cols<N>(st.k[q], 4 * (j >> 1) + i, j & 1, lane);
+                    qt[j & 1][i][q] = tile_cols<N>(st.q[q], 4 * (j >> 1) + i, j & 1, lane);
+                }
+        };
+        cols(0);
+        const float end = fac[kFacEnd];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+            if (j + 1 < NT / 2) cols(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            mma_rows<4, KP, kNP>(kt[j & 1], xs[j & 1], S + 4 * (j >> 1));
+            mma_rows<4, KP, kNP>(qt[j & 1], ys[j & 1], S + 4 * (j >> 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    for (int t = len - 1; t >= 0; --t) {
-        const size_t tok = b * L + t, th = tok * a.heads + h;
-        const float *cur = st + static_cast<size_t>(t) * PN;
-        load_kq(tok);
-        const float beta = a.beta[th], al = expf(clamp_decay(a.g[th]));
-        float sb = 0.f;
-        for (int p = tid; p < P; p += kThreads) {
-            const float dy = a.scale * ldf(static_cast<const T *>(gr.dy) + th * P + p);
-            float d = 0.f, du = 0.f;
-            for (int i = 0; i < N; ++i) {
-                d += cur[p * N + i] * kv[i];
-                ds[p * N + i] += dy * qv[i];
-                du += ds[p * N + i] * kv[i];
-            }
-            const float e = ldf(static_cast<const T *>(a.v) + tok * a.vs + h * P + p) - d;
-            sb += du * e;
-            uv[p] = beta * e;
-            ev[p] = beta * du;
-            yv[p] = dy;
-            stf(static_cast<T *>(gr.dv) + th * P + p, beta * du);
+    if (p >= P) return;
+    for (int t = len + g; t < L; t += 4) stf(dvp + t * pv + p, 0.f);
+    if (gr.dstate0 == nullptr) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = state_n(nt, g, r);
+            if (n < n_of) gr.dstate0[(bh * P + p) * n_of + n] = S[nt][r];
         }
-        sb = block_sum(sb, red);   // its barriers also publish uv, ev, yv and dS
-        for (int i = tid; i < N; i += kThreads) {
-            float dq = 0.f, dk = 0.f;
-            for (int p = 0; p < P; ++p) {
-                dq += yv[p] * (cur[p * N + i] + uv[p] * kv[i]);
-                dk += ds[p * N + i] * uv[p] - cur[p * N + i] * ev[p];
-            }
-            dqh[th * N + i] = dq;
-            dkh[th * N + i] = dk;
+}
+
+// Sums over the sixteen lanes that hold a row of an accumulator tile.
+__device__ __forceinline__ float row16(float v) {
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+template <int DIR>   // inclusive, 1: from lane 0 on, -1: from lane 63 down
+__device__ __forceinline__ double wave_scan(double v, int lane) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double o = DIR > 0 ? __shfl_up(v, off, 64) : __shfl_down(v, off, 64);
+        if (DIR > 0 ? lane >= off : lane + off < 64) v += o;
+    }
+    return v;
+}
+
+// One workgroup a (sequence, group, chunk), a wave sixteen of its tokens; the
+// heads that share the group's q and k in turn, their dq and dk summed in
+// registers.
+template <typename T, int N, bool VEC>
+__global__ void __launch_bounds__(256)
+delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chunks, const float *kept) {
+    constexpr int KP = Parts<T>::in, OP = Parts<T>::out, NT = N / 16;
+    constexpr int s_bytes = kNP * Tile<N>::bytes / 2, xy_bytes = 2 * OP * Tile<64>::bytes, LW = kC + 1;
+    constexpr int region = s_bytes > xy_bytes ? s_bytes : xy_bytes;
+    static_assert(region >= kC * LW * 4, "V shares the region");
+    __shared__ __attribute__((aligned(16))) unsigned char sk[KP][Tile<N>::bytes], sq[KP][Tile<N>::bytes];
+    __shared__ __attribute__((aligned(16))) unsigned char area[region];
+    __shared__ double G[kC];
+    __shared__ float beta[kC], rq[kC], rk[kC], da[kC], db[kC], dks[kC], dots[4];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const size_t id = blockIdx.x, ck = id % chunks, kg = id / chunks % a.groups, b = id / chunks / a.groups;
+    const int L = static_cast<int>(a.seq), t0 = static_cast<int>(ck) * kC, left = L - t0;
+    const int live = valid_len(a.lengths, b, L) - t0;
+    const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
+    const size_t rep = a.heads / a.groups, qk = a.groups * n_of, out0 = (b * L + t0) * qk + kg * n_of;
+    T *dqp = static_cast<T *>(gr.dq) + out0, *dkp = static_cast<T *>(gr.dk) + out0;
+    if (live <= 0) {   // padding: zeros
+        const int rows = left < kC ? left : kC;
+        for (int i = tid; i < rows * n_of; i += 256) {
+            stf(dqp + (i / n_of) * qk + i % n_of, 0.f);
+            stf(dkp + (i / n_of) * qk + i % n_of, 0.f);
         }
-        __syncthreads();
-        float sg = 0.f;
-        for (int p = tid; p < P; p += kThreads)
-            for (int i = 0; i < N; ++i) {
-                const float x = ds[p * N + i] - ev[p] * kv[i];
-                sg += x * cur[p * N + i];
-                ds[p * N + i] = al * x;
+        for (int i = tid; i < rows * static_cast<int>(rep); i += 256) {
+            const size_t th = (b * L + t0 + i / rep) * a.heads + kg * rep + i % rep;
+            gr.dg[th] = gr.dbeta[th] = 0.f;
+        }
+        return;
+    }
+    const Kept kd(a);
+    // the group's rows, and the factors that bring them to unit length
+    {
+        const Rows<T, VEC> kr(static_cast<const T *>(a.k) + (b * L + t0) * a.ks + kg * n_of, a.ks, live, n_of);
+        const Rows<T, VEC> qr(static_cast<const T *>(a.q) + (b * L + t0) * a.qs + kg * n_of, a.qs, live, n_of);
+        constexpr int per = N / 8;   // threads of a row
+#pragma unroll
+        for (int i = 0; i < kC * N / 8 / 256; ++i) {
+            const int t = tid / per + i * (256 / per), n = tid % per * 8;
+            const Eight<T> k8 = load_eight(kr, t, n), q8 = load_eight(qr, t, n);
+            float f[8], ssk = 0.f, ssq = 0.f;
+            widen(k8, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ssk += f[j] * f[j];
+            widen(q8, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ssq += f[j] * f[j];
+#pragma unroll
+            for (int off = 1; off < per; off <<= 1) {
+                ssk += __shfl_xor(ssk, off, 64);
+                ssq += __shfl_xor(ssq, off, 64);
             }
-        sg = block_sum(sg, red);
-        if (tid == 0) {
-            gr.dg[th] = sg;
-            gr.dbeta[th] = sb;
+            if (n == 0) {
+                rk[t] = a.qk_norm ? 1.0f / sqrtf(ssk + kUnitEps) : 1.0f;
+                rq[t] = a.qk_norm ? 1.0f / sqrtf(ssq + kUnitEps) : 1.0f;
+            }
+            bf16x8 x[KP];
+            to_parts(k8, x);
+#pragma unroll
+            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(sk[q] + tile_at<N>(t, n / 8)) = x[q];
+            to_parts(q8, x);
+#pragma unroll
+            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(sq[q] + tile_at<N>(t, n / 8)) = x[q];
         }
     }
     __syncthreads();
-    if (gr.dstate0)
-        for (int i = tid; i < PN; i += kThreads) gr.dstate0[bh * PN + i] = ds[i];
-}
-
-// One wave a (token, group).
-template <typename T>
-__global__ void __launch_bounds__(64) delta_backward_heads(DeltaLaunch a, DeltaGrads gr, const float *dqh, const float *dkh) {
-    const size_t tg = blockIdx.x, tok = tg / a.groups, kg = tg % a.groups, rep = a.heads / a.groups;
-    const int N = static_cast<int>(a.d_state), lane = threadIdx.x;
-    for (int which = 0; which < 2; ++which) {
-        const float *src = (which ? dkh : dqh) + (tok * a.heads + kg * rep) * N;
-        const T *x = which ? static_cast<const T *>(a.k) + tok * a.ks + kg * N
-                           : static_cast<const T *>(a.q) + tok * a.qs + kg * N;
-        T *out = static_cast<T *>(which ? gr.dk : gr.dq) + tg * N;
-        float d[4], xv[4], ss = 0.f, sd = 0.f;
+    f32x4 dq[NT], dk[NT], qkt[4], kkt[4];
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) dq[nt] = dk[nt] = zero;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) qkt[j] = kkt[j] = zero;
+#pragma unroll
+    for (int kk = 0; kk < N / 32; ++kk) {
+        bf16x8 qa[KP], ka[KP], kb[KP];
+#pragma unroll
+        for (int q = 0; q < KP; ++q) {
+            qa[q] = tile_rows<N>(sq[q], w, kk, lane);
+            ka[q] = tile_rows<N>(sk[q], w, kk, lane);
+        }
+#pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int n = lane + 64 * j;
-            d[j] = xv[j] = 0.f;
-            if (n >= N) continue;
-            for (size_t r = 0; r < rep; ++r) d[j] += src[r * N + n];
-            xv[j] = ldf(x + n);
-            ss += xv[j] * xv[j];
-            sd += xv[j] * d[j];
+            if (j > w) continue;
+#pragma unroll
+            for (int q = 0; q < KP; ++q) kb[q] = tile_rows<N>(sk[q], j, kk, lane);
+            qkt[j] = mma_parts<KP, KP>(qa, kb, qkt[j]);
+            kkt[j] = mma_parts<KP, KP>(ka, kb, kkt[j]);
         }
-        float r = 1.f, c = 0.f;
-        if (a.qk_norm) {
-            r = 1.0f / sqrtf(group_sum(ss, 64) + kUnitEps);
-            c = group_sum(sd, 64) * r * r;
+    }
+    // q (or k) of this lane's place r of tile nt, from its parts
+    const auto value = [&](const unsigned char(*t)[Tile<N>::bytes], int nt, int r) {
+        const int at = tile_at<N>(16 * w + 4 * g + r, 4 * (nt >> 1) + (c >> 2)) + 8 * (nt & 1) + 2 * (c & 3);
+        float v = 0.f;
+#pragma unroll
+        for (int q = KP - 1; q >= 0; --q) v += bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(t[q] + at));
+        return v;
+    };
+    for (size_t hr = 0; hr < rep; ++hr) {
+        const size_t h = kg * rep + hr, rec = (b * a.heads + h) * chunks + ck;
+        const float *fac = reinterpret_cast<const float *>(records + rec * (BackRecord::units * 1024));
+        const float *keep = kept + rec * kd.floats();
+        const Rows<T, VEC> dyr(static_cast<const T *>(gr.dy) + ((b * L + t0) * a.heads + h) * P, a.heads * P, live, P);
+        if (w == 0) {
+            const size_t th = (b * L + t0 + lane) * a.heads + h;
+            G[lane] = wave_scan<1>(lane < live ? static_cast<double>(clamp_decay(a.g[th])) : 0.0, lane);
+            beta[lane] = lane < live ? a.beta[th] : 0.f;
         }
+        f32x4 qi[NT], ki[NT], ks[NT], f[4], z[4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) qi[nt] = ki[nt] = ks[nt] = zero;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = z[j] = zero;
+        float dot = 0.f;   // of S0 and dS1
+        for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
+            constexpr int pieces = 32 * N / 8 / 256, per = N / 8;
+            const int pr = tid / per, pn = tid % per * 8;
+            float s0[pieces][8], s1[pieces][8];
+#pragma unroll
+            for (int i = 0; i < pieces; ++i) {
+                const float *s = keep + (pb + pr + i * (256 / per)) * N + pn;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const f32x4 x0 = *reinterpret_cast<const f32x4 *>(s + kd.s0() + 4 * v);
+                    const f32x4 x1 = *reinterpret_cast<const f32x4 *>(s + kd.s1() + 4 * v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s0[i][4 * v + j] = x0[j];
+                        s1[i][4 * v + j] = x1[j];
+                        dot += x0[j] * x1[j];
+                    }
+                }
+            }
+            // rows of dY, dR, E: columns pb + 4g .. and pb + 16 + 4g ..
+            const auto kept_row = [&](size_t at, int t, bf16x8 *out) {
+                const float *s = keep + at + t * kd.p64 + pb + 4 * g;
+                split_tiles<kNP>(*reinterpret_cast<const f32x4 *>(s), *reinterpret_cast<const f32x4 *>(s + 16), out);
+            };
+            bf16x8 ya[KP], ra[kNP], ea[kNP];
+            {
+                float y8[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
+                    y8[j] = value_of<T>(load_one(dyr, row_off<T>(dyr.stride, P, 16 * w + c, n), 16 * w + c, n, 0));
+                }
+                split8<KP>(y8, ya);
+            }
+            kept_row(kd.dr(), 16 * w + c, ra);
+            kept_row(kd.e(), 16 * w + c, ea);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > w) continue;
+                bf16x8 eb[kNP];
+                kept_row(kd.e(), 16 * j + c, eb);
+                f[j] = mma_parts<KP, kNP>(ya, eb, f[j]);
+                z[j] = mma_parts<kNP, kNP>(ra, eb, z[j]);
+            }
+            const auto put = [&](const float(*s)[8]) {
+#pragma unroll
+                for (int i = 0; i < pieces; ++i) {
+                    bf16x8 x[kNP];
+                    split8<kNP>(s[i], x);
+#pragma unroll
+                    for (int q = 0; q < kNP; ++q)
+                        *reinterpret_cast<bf16x8 *>(area + q * (Tile<N>::bytes / 2) +
+                                                    tile_at<N>(pr + i * (256 / per), pn / 8)) = x[q];
+                }
+            };
+            const auto state = [&](int nt, bf16x8 *out) {
+#pragma unroll
+                for (int q = 0; q < kNP; ++q) out[q] = tile_cols<N>(area + q * (Tile<N>::bytes / 2), nt, 0, lane);
+            };
+            __syncthreads();
+            put(s0);
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                bf16x8 s[kNP];
+                state(nt, s);
+                qi[nt] = mma_parts<KP, kNP>(ya, s, qi[nt]);
+                ki[nt] = mma_parts<kNP, kNP>(ra, s, ki[nt]);
+            }
+            __syncthreads();
+            put(s1);
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                bf16x8 s[kNP];
+                state(nt, s);
+                ks[nt] = mma_parts<kNP, kNP>(ea, s, ks[nt]);
+            }
+        }
+        dot = group_sum(dot, 64);
+        if (lane == 0) dots[w] = dot;
+        // row by row: what the states contribute
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int t = 16 * w + 4 * g + r;
+            const float fq = fac[kFacQ + t], fk = fac[kFacK + t], fu = fac[kFacU + t];
+            float xq = 0.f, xk = 0.f, xs = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float kv = value(sk, nt, r);
+                xq += value(sq, nt, r) * qi[nt][r];
+                xk += kv * ki[nt][r];
+                xs += kv * ks[nt][r];
+                dq[nt][r] += fq * qi[nt][r];
+                dk[nt][r] += fu * ks[nt][r] - fk * ki[nt][r];
+            }
+            xq = row16(xq);
+            xk = row16(xk);
+            xs = row16(xs);
+            if (c == 0) {
+                da[t] = fq * xq - fk * xk;
+                db[t] = fu * xs;
+                dks[t] = rk[t] * xs;
+            }
+        }
+        // the triangle
+        __syncthreads();
+        float(*V)[LW] = reinterpret_cast<float(*)[LW]>(area);
+#pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < N)
-                // d == 0: a padding token, whatever it holds
-                stf(out + lane + 64 * j, d[j] == 0.f && c != c ? 0.f : r * (d[j] - xv[j] * c));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * w + 4 * g + r, jj = 16 * j + c;
+                float x = 0.f, y = 0.f, v = 0.f;
+                if (jj <= i) {
+                    const float d = expf(static_cast<float>(G[i] - G[jj])) * rk[jj];
+                    x = a.scale * rq[i] * d * f[j][r];
+                    if (jj < i) y = rk[i] * d * z[j][r];
+                    v = x * qkt[j][r] - y * kkt[j][r];
+                }
+                V[i][jj] = v;
+                f[j][r] = x * beta[jj];
+                z[j][r] = -y * beta[jj];
+            }
+        __syncthreads();
+        if (w == 0) {
+            const int t = lane;
+            double col = 0.0, all = 0.0, row = 0.0;
+            for (int i = 0; i < kC; ++i) {
+                const double v = V[i][t];
+                if (i > t) col += v;
+                if (i >= t) all += v;
+                if (i < t) row += static_cast<double>(beta[i]) * V[t][i];
+            }
+            const double up = wave_scan<-1>(row - beta[t] * col + da[t], lane);
+            const double down = wave_scan<1>(db[t], lane) - db[t];
+            const float dot_all = dots[0] + dots[1] + dots[2] + dots[3];
+            const size_t th = (b * L + t0 + t) * a.heads + h;
+            if (t < left) {
+                const bool ok = t < live;
+                gr.dg[th] = ok ? static_cast<float>(up + down + static_cast<double>(fac[kFacEnd]) * dot_all) : 0.f;
+                gr.dbeta[th] = ok ? static_cast<float>(all + expf(static_cast<float>(G[kC - 1] - G[t])) * dks[t]) : 0.f;
+            }
+        }
+        __syncthreads();
+        // X and -Y as parts, then the products within the chunk
+        const auto place = [&](int which, int q) { return area + (which * OP + q) * Tile<64>::bytes; };
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * w + 4 * g + r;
+                const int at = tile_at<64>(i, 2 * j + (c >> 3)) + 2 * (c & 7);
+                float x = f[j][r], y = z[j][r];
+#pragma unroll
+                for (int q = 0; q < OP; ++q) {
+                    const bf16_t xb = from_f32<bf16_t>(x), yb = from_f32<bf16_t>(y);
+                    *reinterpret_cast<uint16_t *>(place(0, q) + at) = xb.bits;
+                    *reinterpret_cast<uint16_t *>(place(1, q) + at) = yb.bits;
+                    x -= to_f32(xb);
+                    y -= to_f32(yb);
+                }
+            }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            // rows 16 w of X and Y (tokens 32 kk + 4g .., + 16 + 4g ..), and of their transposes
+            bf16x8 xr[OP], yr[OP], xt[OP], yt[OP];
+#pragma unroll
+            for (int q = 0; q < OP; ++q) {
+                const int piece = 4 * kk + (g >> 1), off = 8 * (g & 1), t = 16 * w + c;
+                const auto four = [&](int which, int pc) {
+                    return *reinterpret_cast<const bf16x4 *>(place(which, q) + tile_at<64>(t, pc) + off);
+                };
+                xr[q] = __builtin_shufflevector(four(0, piece), four(0, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
+                yr[q] = __builtin_shufflevector(four(1, piece), four(1, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
+                const auto acc = [&](int which, int i) { return tile_acc(place(which, q), i, w, lane); };
+                xt[q] = __builtin_shufflevector(acc(0, 2 * kk), acc(0, 2 * kk + 1), 0, 1, 2, 3, 4, 5, 6, 7);
+                yt[q] = __builtin_shufflevector(acc(1, 2 * kk), acc(1, 2 * kk + 1), 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                bf16x8 kc[KP], qc[KP];
+#pragma unroll
+                for (int q = 0; q < KP; ++q) {
+                    kc[q] = tile_cols<N>(sk[q], nt, kk, lane);
+                    qc[q] = tile_cols<N>(sq[q], nt, kk, lane);
+                }
+                if (kk <= (w >> 1)) {
+                    dq[nt] = mma_parts<OP, KP>(xr, kc, dq[nt]);
+                    dk[nt] = mma_parts<OP, KP>(yr, kc, dk[nt]);
+                }
+                if (kk >= (w >> 1)) {
+                    dk[nt] = mma_parts<OP, KP>(xt, qc, dk[nt]);
+                    dk[nt] = mma_parts<OP, KP>(yt, kc, dk[nt]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // through the norm, and out
+    const Rows<T, VEC> dqr(dqp, qk, left, n_of), dkr(dkp, qk, left, n_of);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = 16 * w + 4 * g + r;
+        float xq = 0.f, xk = 0.f;
+        if (a.qk_norm) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                xq += value(sq, nt, r) * dq[nt][r];
+                xk += value(sk, nt, r) * dk[nt][r];
+            }
+            xq = row16(xq) * rq[t] * rq[t];
+            xk = row16(xk) * rk[t] * rk[t];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int n = state_n(nt, c >> 2, c & 3);
+            const uint32_t at = row_off<T>(qk, n_of, t, n);
+            store_one(dqr, at, t, n, 0, dq[nt][r] - value(sq, nt, r) * xq);
+            store_one(dkr, at, t, n, 0, dk[nt][r] - value(sk, nt, r) * xk);
+        }
     }
 }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-}  // namespace
-
-size_t delta_backward_workspace(const DeltaLaunch &a) {
-    const size_t pn = a.head_dim * a.d_state, bh = a.batch * a.heads;
-    return align256(bh * a.seq * pn * 4) + 2 * align256(bh * a.seq * a.d_state * 4) + align256(bh * pn * 4);
+size_t records_bytes(const DeltaLaunch &a) {
+    return align256(a.batch * a.heads * chunks_of(a) * BackRecord::units * 1024);
 }
 
-hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void *workspace,
-                                 hipStream_t s, int &launches) {
-    const size_t pn = a.head_dim * a.d_state, bh = a.batch * a.heads;
-    char *w = static_cast<char *>(workspace);
-    float *states = reinterpret_cast<float *>(w);
-    w += align256(bh * a.seq * pn * 4);
-    float *dqh = reinterpret_cast<float *>(w);
-    w += align256(bh * a.seq * a.d_state * 4);
-    float *dkh = reinterpret_cast<float *>(w);
-    w += align256(bh * a.seq * a.d_state * 4);
-    float *dS = reinterpret_cast<float *>(w);
-    const size_t lds = (2 * a.d_state + 3 * a.head_dim) * 4;
+}  // namespace
+
+bool delta_backward_supported(const DeltaLaunch &a) { return a.d_state <= 128; }
+
+size_t delta_backward_workspace(const DeltaLaunch &a) {
+    return records_bytes(a) + a.batch * a.heads * chunks_of(a) * Kept(a).floats() * sizeof(float);
+}
+
+hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void *workspace, hipStream_t s,
+                                 int &launches) {
+    unsigned char *records = static_cast<unsigned char *>(workspace);
+    float *kept = reinterpret_cast<float *>(records + records_bytes(a));
+    if (a.seq > 0) {
+        const hipError_t e = launch_delta_states(a, records, kept, s, launches);
+        if (e != hipSuccess) return e;
+    }
     return by_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        if (bh == 0) return hipSuccess;
-        hipLaunchKernelGGL(delta_backward_walk<T>, dim3(static_cast<unsigned>(bh)), dim3(kThreads), lds, s, a,
-                           g, states, dqh, dkh, dS);
-        ++launches;
-        if (a.seq > 0) {
-            hipLaunchKernelGGL(delta_backward_heads<T>, dim3(static_cast<unsigned>(a.batch * a.seq * a.groups)),
-                               dim3(64), 0, s, a, g, dqh, dkh);
-            ++launches;
-        }
-        return hipGetLastError();
+        return by_state(a.d_state, [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            const int chunks = static_cast<int>(chunks_of(a));
+            const dim3 rev(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>((a.head_dim + 63) / 64));
+            const dim3 own(static_cast<unsigned>(a.batch * a.groups * chunks));
+            const auto go = [&](auto vec) {
+                constexpr bool VEC = decltype(vec)::value;
+                hipLaunchKernelGGL((delta_reverse<T, N, VEC>), rev, dim3(256), 0, s, a, g, records, chunks, kept);
+                ++launches;
+                if (chunks > 0) {
+                    hipLaunchKernelGGL((delta_grads<T, N, VEC>), own, dim3(256), 0, s, a, g, records, chunks, kept);
+                    ++launches;
+                }
+                return hipGetLastError();
+            };
+            // the gradients' rows are as v's and y's, q's and k's contiguous ones
+            DeltaLaunch o = a;
+            o.y = const_cast<void *>(g.dy);
+            bool vec = rows_vec(o, sizeof(T));
+            o.y = g.dv;
+            o.q = g.dq;
+            o.k = g.dk;
+            o.qs = o.ks = a.groups * a.d_state;
+            vec = vec && rows_vec(o, sizeof(T));
+            return vec ? go(std::true_type{}) : go(std::false_type{});
+        });
     });
 }
 

@@ -9,10 +9,11 @@ using namespace delta;
 
 // One workgroup a (sequence, head, chunk): the chunk's row factors, T and the
 // attention within the chunk.
-template <typename T, int N, bool VEC>
+template <typename T, int N, bool VEC, bool BACK>
 __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *records, int chunks) {
     constexpr int KP = Parts<T>::in, LP = kC + 4;
     using R = Record<T>;
+    constexpr size_t bytes = (BACK ? BackRecord::units : R::units) * 1024;
     __shared__ double G[kC];
     __shared__ float beta[kC], rq[kC], rk[kC];
     __shared__ __attribute__((aligned(16))) float A[kC][LP], X[kC][LP];
@@ -97,36 +98,41 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
             A[i][jj] = m;
             X[i][jj] = p;
         }
-    unsigned char *out = records + rec * R::bytes;
+    unsigned char *out = records + rec * bytes;
     if (w == 0) {
         float *f = reinterpret_cast<float *>(out);
         const float eg = expf(static_cast<float>(G[lane]));
-        f[R::kK + lane] = eg * rk[lane];
-        f[R::kQ + lane] = eg * rq[lane];
-        f[R::kU + lane] = beta[lane] * expf(static_cast<float>(G[kC - 1] - G[lane])) * rk[lane];
-        if (lane == 0) f[R::kEnd] = expf(static_cast<float>(G[kC - 1]));
+        f[kFacK + lane] = eg * rk[lane];
+        f[kFacQ + lane] = eg * rq[lane];
+        f[kFacU + lane] = beta[lane] * expf(static_cast<float>(G[kC - 1] - G[lane])) * rk[lane];
+        if (lane == 0) f[kFacEnd] = expf(static_cast<float>(G[kC - 1]));
     }
     __syncthreads();
-    // a triangle of X or A as operand blocks: wave w writes those of rows 16 w
-    const auto emit = [&](const float(*src)[LP], unsigned char *dst, auto parts) {
+    // a triangle of X as operand blocks, or of its transpose: wave w writes those
+    // of rows 16 w
+    const auto emit = [&](int unit, auto parts, auto upper) {
         constexpr int NP = decltype(parts)::value;
-        for (int kk = 0; kk < lower_steps(w); ++kk) {
+        constexpr bool UP = decltype(upper)::value;
+        for (int kk = UP ? w >> 1 : 0; kk < (UP ? 2 : 1 + (w >> 1)); ++kk) {
             float x[8];
-            const f32x4 lo = *reinterpret_cast<const f32x4 *>(&src[my][32 * kk + 4 * g]);
-            const f32x4 hi = *reinterpret_cast<const f32x4 *>(&src[my][32 * kk + 16 + 4 * g]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = lo[i];
-                x[4 + i] = hi[i];
+            for (int i = 0; i < 8; ++i) {
+                const int k = 32 * kk + 16 * (i >> 2) + 4 * g + (i & 3);
+                x[i] = UP ? X[k][my] : X[my][k];
             }
             bf16x8 o[NP];
             split8<NP>(x, o);
+            const int blk = UP ? upper_block(w, kk) : lower_block(w, kk);
 #pragma unroll
             for (int p = 0; p < NP; ++p)
-                *reinterpret_cast<bf16x8 *>(dst + ((lower_block(w, kk) * NP + p) * 64 + lane) * 16) = o[p];
+                *reinterpret_cast<bf16x8 *>(out + unit * 1024 + ((blk * NP + p) * 64 + lane) * 16) = o[p];
         }
     };
-    emit(X, out + R::p_at, std::integral_constant<int, Parts<T>::out>{});
+    constexpr std::integral_constant<int, kNP> full{};
+    if constexpr (BACK)
+        emit(BackRecord::pt, full, std::true_type{});
+    else
+        emit(R::p, std::integral_constant<int, Parts<T>::out>{}, std::false_type{});
     // T = (I + A)^-1.  The diagonal blocks by substitution, wave w block w, a
     // column a lane (the four lane groups alike)
     {
@@ -174,48 +180,37 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
                 for (int r = 0; r < 4; ++r) X[16 * (w + d) + 4 * g + r][16 * w + c] = t[d][r];
     }
     // above the diagonal T is zero where a block row's operands reach past it
-    if (w < 4) {
-        const int j = w ^ 1;   // the other half of this row's last block pair
-        if (j > w)
+    if ((w & 1) == 0)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) X[16 * w + 4 * g + r][16 * j + c] = 0.f;
-    }
+        for (int r = 0; r < 4; ++r) X[16 * w + 4 * g + r][16 * (w + 1) + c] = 0.f;
     __syncthreads();
-    emit(X, out + R::t_at, std::integral_constant<int, kNP>{});
+    emit(R::t, full, std::false_type{});
+    if constexpr (BACK) emit(BackRecord::tt, full, std::true_type{});
 }
 
-// A chunk's operands in LDS.
-template <typename T, int N> struct Staged {
-    unsigned char k[Parts<T>::in][Tile<N>::bytes], q[Parts<T>::in][Tile<N>::bytes];
-    unsigned char v[sizeof(T) == 2 ? Tile<64>::bytes : 16];
-    unsigned char rec[Record<T>::bytes];
-};
-
 // One workgroup a (sequence, head, 64 columns of P), a wave 16 of them, the
-// chunks in turn.  bf16 with aligned rows: a chunk's operands go straight from
-// memory to LDS while the one before is multiplied (two buffers, one barrier a
-// chunk).  Other inputs become their bf16 parts on the way: through registers
-// into one buffer.
-template <typename T, int N, bool VEC>
+// chunks in turn.  With KEEP, the backward's way in: no y, but the state before
+// each chunk and its E are kept.
+template <typename T, int N, bool VEC, bool KEEP>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
+delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept) {
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 32, NT = N / 16;
-    constexpr bool DMA = VEC && std::is_same<T, bf16_t>::value;
     using R = Record<T>;
-    constexpr int pieces = kC * N / 8 / 256, rpieces = (R::bytes / 16 + 255) / 256;
-    __shared__ __attribute__((aligned(1024))) Staged<T, N> staged[DMA ? 2 : 1];
-    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA ? 4 : 1][DMA ? kC : 1][16];
-    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, kg = h / (a.heads / a.groups);
+    constexpr size_t rec_bytes = (KEEP ? BackRecord::units : R::units) * 1024;
+    using St = Stage<T, N, VEC, !KEEP, KEEP ? R::p : R::units, 0>;
+    constexpr bool DMA = St::DMA;
+    __shared__ __attribute__((aligned(1024))) typename St::Buf staged[DMA ? 2 : 1];
+    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && !KEEP ? 4 : 1][DMA && !KEEP ? kC : 1][16];
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
     const int p0 = blockIdx.y * 64, p = p0 + 16 * w + c;      // this lane's column
-    const T *kp = static_cast<const T *>(a.k) + b * L * a.ks + kg * n_of;
-    const T *qp = static_cast<const T *>(a.q) + b * L * a.qs + kg * n_of;
-    const T *vp = static_cast<const T *>(a.v) + b * L * a.vs + h * P;
     T *yp = static_cast<T *>(a.y) + (b * L * a.heads + h) * P;
     const size_t ystep = a.heads * P;
+    const uint32_t y_at = row_off<T>(ystep, P, 4 * g, p);
+    const Kept kd(a);
     f32x4 S[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -225,91 +220,35 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
             S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
         }
     const int live = (len + kC - 1) / kC;
-    // the fetch of a chunk, in four parts; DMA: to LDS
-    const uint32_t dk = dma_at<T, N>(a.ks, n_of, 0, w, lane), dq = dma_at<T, N>(a.qs, n_of, 0, w, lane);
-    const uint32_t dv = dma_at<T, 64>(a.vs, P, p0, w, lane);
-    const auto dma = [&](int ck, int part) {
-        Staged<T, N> &to = staged[DMA ? ck & 1 : 0];
-        const size_t t0 = static_cast<size_t>(ck) * kC;
-        const int left = len - ck * kC;
-        if (part == 0) dma_tile<N>(Rows<T, true>(kp + t0 * a.ks, a.ks, left, n_of), dk, to.k[0], w);
-        if (part == 1) dma_tile<N>(Rows<T, true>(qp + t0 * a.qs, a.qs, left, n_of), dq, to.q[0], w);
-        if (part == 2) dma_tile<64>(Rows<T, true>(vp + t0 * a.vs, a.vs, left, P), dv, to.v, w);
-        if (part >= 2) {
-            const rsrc_t rec = make_rsrc(records + (bh * chunks + ck) * R::bytes, R::bytes);
-            constexpr int units = R::bytes / 1024, half = (units + 7) / 8;
-#pragma unroll
-            for (int i = 0; i < half; ++i) {
-                const int u = w + 4 * (i + (part - 2) * half);
-                if (u < units) scan::lds_dma16(rec, scan::lds_addr(to.rec + u * 1024), u * 1024 + lane * 16);
-            }
-        }
-    };
-    // else: to registers
-    const int kt0 = tid / (N / 8), kn = tid % (N / 8) * 8;
-    const uint32_t k_at = row_off<T>(a.ks, n_of, kt0, kn), q_at = row_off<T>(a.qs, n_of, kt0, kn);
-    const uint32_t v_at = row_off<T>(a.vs, P, 4 * g, p), y_at = row_off<T>(ystep, P, 4 * g, p);
-    Eight<T> k8[pieces], q8[pieces];
-    u32x4 r8[rpieces];
-    uint32_t v[4][4];
-    const auto fetch = [&](int ck) {
-        const size_t t0 = static_cast<size_t>(ck) * kC;
-        const int left = len - ck * kC;
-        const Rows<T, VEC> kr(kp + t0 * a.ks, a.ks, left, n_of), qr(qp + t0 * a.qs, a.qs, left, n_of);
-        const Rows<T, VEC> vr(vp + t0 * a.vs, a.vs, left, P);
-#pragma unroll
-        for (int i = 0; i < pieces; ++i) {
-            k8[i] = load_eight(kr, k_at, kt0, kn, i * (2048 / N));
-            q8[i] = load_eight(qr, q_at, kt0, kn, i * (2048 / N));
-        }
-        const rsrc_t rec = make_rsrc(records + (bh * chunks + ck) * R::bytes, R::bytes);
-#pragma unroll
-        for (int i = 0; i < rpieces; ++i) r8[i] = bld16(rec, (tid + 256 * i) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[i][r] = load_one(vr, v_at, 4 * g, p, 16 * i + r);
-    };
-    const auto put = [&]() {
-#pragma unroll
-        for (int i = 0; i < pieces; ++i) {
-            bf16x8 x[KP];
-            const int at = tile_at<N>(kt0 + i * (2048 / N), kn / 8);
-            to_parts(k8[i], x);
-#pragma unroll
-            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(staged[0].k[q] + at) = x[q];
-            to_parts(q8[i], x);
-#pragma unroll
-            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(staged[0].q[q] + at) = x[q];
-        }
-#pragma unroll
-        for (int i = 0; i < rpieces; ++i)
-            if (tid + 256 * i < static_cast<int>(R::bytes / 16))
-                reinterpret_cast<u32x4 *>(staged[0].rec)[tid + 256 * i] = r8[i];
-    };
+    St in(a, b, h, len, static_cast<const T *>(a.v) + b * L * a.vs + h * P, a.vs, p0,
+          records + bh * chunks * rec_bytes, rec_bytes);
     if (live > 0) {
         if constexpr (DMA) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dma(0, i);
+            for (int i = 0; i < 4; ++i) in.dma(staged[0], 0, i);
         } else {
-            fetch(0);
+            in.fetch(0);
         }
     }
     for (int ck = 0; ck < live; ++ck) {
-        const Staged<T, N> &st = staged[DMA ? ck & 1 : 0];
+        typename St::Buf &st = staged[DMA ? ck & 1 : 0], &next = staged[DMA ? (ck + 1) & 1 : 0];
         f32x4 e[4];
         if constexpr (DMA) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         } else {
             __syncthreads();
-            put();
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) e[i][r] = value_of<T>(v[i][r]);
+            in.put(st);
+            in.values(st, e);
             __syncthreads();
-            if (ck + 1 < live) fetch(ck + 1);
+            if (ck + 1 < live) in.fetch(ck + 1);
+        }
+        float *keep = nullptr;
+        if constexpr (KEEP) {
+            keep = kept + (bh * chunks + ck) * kd.floats();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                *reinterpret_cast<f32x4 *>(keep + kd.s0() + p * N + state_n(nt, g, 0)) = S[nt];
         }
         const float *fac = reinterpret_cast<const float *>(st.rec);
         // R and the state's part of Y: while a k-step is multiplied, the next one's
@@ -324,13 +263,8 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
 #pragma unroll
                 for (int q = 0; q < KP; ++q) {
                     kf[kk & 1][i][q] = tile_rows<N>(st.k[q], i, kk, lane);
-                    qf[kk & 1][i][q] = tile_rows<N>(st.q[q], i, kk, lane);
+                    if constexpr (!KEEP) qf[kk & 1][i][q] = tile_rows<N>(st.q[q], i, kk, lane);
                 }
-        };
-        // blocks of a triangle: those of the first k-step, then the second's
-        constexpr int at4[4] = {0, 1, 2, 4}, at2[2] = {3, 5};
-        const auto tri = [&](size_t at, int np, int blk, int q) {
-            return *reinterpret_cast<const bf16x8 *>(st.rec + at + ((blk * np + q) * 64 + lane) * 16);
         };
         bf16x8 t4[4][kNP], t2[2][kNP];
         rows(0);
@@ -340,40 +274,25 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
             if (kk + 1 < KS) {
                 rows(kk + 1);
             } else {
-#pragma unroll
-                for (int q = 0; q < kNP; ++q) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t4[i][q] = tri(R::t_at, kNP, at4[i], q);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) t2[i][q] = tri(R::t_at, kNP, at2[i], q);
-                }
-                if constexpr (DMA) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bf16x4 x = tile_acc(st.v, i, w, lane);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) e[i][r] = static_cast<float>(x[r]);
-                    }
-                }
+                tri_load<kNP>(st.rec + R::t * 1024, lane, t4, t2, false);
+                if constexpr (DMA) in.values(st, e);
             }
             if constexpr (DMA) {
                 if (ck + 1 < live)
 #pragma unroll
-                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) dma(ck + 1, i);
+                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) in.dma(next, ck + 1, i);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
-            mma_rows<4, KP, YP>(qf[kk & 1], sp[kk & 1], y);
+            if constexpr (!KEEP) mma_rows<4, KP, YP>(qf[kk & 1], sp[kk & 1], y);
             interleave<4 * (3 + 2), 3>();
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x4 fk = *reinterpret_cast<const f32x4 *>(fac + R::kK + 16 * i + 4 * g);
-            const f32x4 fq = *reinterpret_cast<const f32x4 *>(fac + R::kQ + 16 * i + 4 * g);
-            e[i] -= fk * ks[i];
-            y[i] *= fq;
+            e[i] -= *reinterpret_cast<const f32x4 *>(fac + kFacK + 16 * i + 4 * g) * ks[i];
+            if constexpr (!KEEP) y[i] *= *reinterpret_cast<const f32x4 *>(fac + kFacQ + 16 * i + 4 * g);
         }
         // E = T R
         bf16x8 x[2][kNP];
@@ -394,37 +313,38 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
                     kt[j & 1][i][q] = tile_cols<N>(st.k[q], 4 * (j >> 1) + i, j & 1, lane);
         };
         cols(0);
-        split_tiles<YP>(e[0], e[1], xe[0]);
-        split_tiles<YP>(e[2], e[3], xe[1]);
+        if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] *= *reinterpret_cast<const f32x4 *>(fac + R::kU + 16 * i + 4 * g);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) keep[kd.e() + (16 * i + 4 * g + r) * kd.p64 + p] = e[i][r];
+        } else {
+            split_tiles<YP>(e[0], e[1], xe[0]);
+            split_tiles<YP>(e[2], e[3], xe[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] *= *reinterpret_cast<const f32x4 *>(fac + kFacU + 16 * i + 4 * g);
         split_tiles<kNP>(e[0], e[1], x[0]);
         split_tiles<kNP>(e[2], e[3], x[1]);
-        const float end = fac[R::kEnd];
+        const float end = fac[kFacEnd];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
 #pragma unroll
         for (int j = 0; j < NT / 2; ++j) {
-            if (j + 1 < NT / 2) {
+            if (j + 1 < NT / 2)
                 cols(j + 1);
-            } else {
-#pragma unroll
-                for (int q = 0; q < YP; ++q) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p4[i][q] = tri(R::p_at, YP, at4[i], q);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) p2[i][q] = tri(R::p_at, YP, at2[i], q);
-                }
-            }
+            else if constexpr (!KEEP)
+                tri_load<YP>(st.rec + R::p * 1024, lane, p4, p2, false);
             __builtin_amdgcn_sched_barrier(0);
             mma_rows<4, KP, kNP>(kt[j & 1], x[j & 1], S + 4 * (j >> 1));
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (KEEP) continue;
         mma_rows<4, YP, YP>(p4, xe[0], y);
         mma_rows<2, YP, YP>(p2, xe[1], y + 2);
         // padding rows past the buffer's end are dropped
         const Rows<T, VEC> yr(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
-        if constexpr (DMA) {
+        if constexpr (DMA && !KEEP) {
             // the wave's 16 columns through LDS to 16-byte stores
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -443,7 +363,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
                 for (int r = 0; r < 4; ++r) store_one(yr, y_at, 4 * g, p, 16 * i + r, y[i][r]);
         }
     }
-    if (p >= P) return;
+    if (KEEP || p >= P) return;
     for (int t = len + g; t < L; t += 4) stf(yp + t * ystep + p, 0.f);
     if (a.state_out == nullptr) return;
 #pragma unroll
@@ -455,15 +375,32 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks) {
         }
 }
 
-template <typename F>
-hipError_t by_state(size_t d_state, F f) {
-    if (d_state <= 64) return f(std::integral_constant<int, 64>{});
-    return f(std::integral_constant<int, 128>{});
+template <bool KEEP>
+hipError_t launch(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s, int &launches) {
+    return by_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        return by_state(a.d_state, [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            const int chunks = static_cast<int>(chunks_of(a));
+            const dim3 prep(static_cast<unsigned>(a.batch * a.heads * chunks));
+            const dim3 main(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>((a.head_dim + 63) / 64));
+            const auto go = [&](auto vec) {
+                constexpr bool VEC = decltype(vec)::value;
+                hipLaunchKernelGGL((delta_prep<T, N, VEC, KEEP>), prep, dim3(256), 0, s, a, records, chunks);
+                hipLaunchKernelGGL((delta_chunks<T, N, VEC, KEEP>), main, dim3(256), 0, s, a, records, chunks, kept);
+                launches += 2;
+                return hipGetLastError();
+            };
+            return rows_vec(a, sizeof(T)) ? go(std::true_type{}) : go(std::false_type{});
+        });
+    });
 }
+
+}  // namespace
 
 // 16-byte access to the rows of q, k, v and y: whole pieces of eight, every row
 // aligned; a chunk's offsets below 2^31.
-bool rows_vec(const DeltaLaunch &a, size_t size) {
+bool delta::rows_vec(const DeltaLaunch &a, size_t size) {
     const auto ok = [&](const void *p, size_t stride) {
         return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0 &&
                (stride + 1024) * size * kC < size_t(1) << 31;
@@ -472,40 +409,24 @@ bool rows_vec(const DeltaLaunch &a, size_t size) {
            ok(a.y, a.heads * a.head_dim);
 }
 
-size_t chunks_of(const DeltaLaunch &a) { return (a.seq + kC - 1) / kC; }
-
-}  // namespace
+hipError_t delta::launch_delta_states(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s,
+                                      int &launches) {
+    return launch<true>(a, records, kept, s, launches);
+}
 
 bool delta_chunk_wanted(const DeltaLaunch &a) { return a.d_state <= 128 && a.seq > 16; }
 
 size_t delta_chunk_workspace(const DeltaLaunch &a) {
     size_t bytes = 0;
     (void)by_type(a.dtype, [&](auto t) {
-        bytes = a.batch * a.heads * chunks_of(a) * Record<decltype(t)>::bytes;
+        bytes = a.batch * a.heads * chunks_of(a) * Record<decltype(t)>::units * 1024;
         return hipSuccess;
     });
     return bytes;
 }
 
 hipError_t launch_delta_chunk(const DeltaLaunch &a, void *workspace, hipStream_t s, int &launches) {
-    return by_type(a.dtype, [&](auto t) {
-        using T = decltype(t);
-        return by_state(a.d_state, [&](auto n) {
-            constexpr int N = decltype(n)::value;
-            const int chunks = static_cast<int>(chunks_of(a));
-            unsigned char *rec = static_cast<unsigned char *>(workspace);
-            const dim3 prep(static_cast<unsigned>(a.batch * a.heads * chunks));
-            const dim3 main(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>((a.head_dim + 63) / 64));
-            const auto go = [&](auto vec) {
-                constexpr bool VEC = decltype(vec)::value;
-                hipLaunchKernelGGL((delta_prep<T, N, VEC>), prep, dim3(256), 0, s, a, rec, chunks);
-                hipLaunchKernelGGL((delta_chunks<T, N, VEC>), main, dim3(256), 0, s, a, rec, chunks);
-                launches += 2;
-                return hipGetLastError();
-            };
-            return rows_vec(a, sizeof(T)) ? go(std::true_type{}) : go(std::false_type{});
-        });
-    });
+    return launch<false>(a, static_cast<unsigned char *>(workspace), nullptr, s, launches);
 }
 
 }  // namespace m3

@@ -291,22 +291,200 @@ __device__ __forceinline__ void dma_tile(const R &rows, uint32_t at, unsigned ch
         scan::lds_dma16(rows.r, scan::lds_addr(tile + (w + 4 * i) * 1024), at + i * (2048 / N) * rows.step);
 }
 
-// Block (i, kk) of a lower-triangular 64 x 64 operand (rows 16 i, columns 32 kk)
-// among its kTri stored ones: 0 .. 1, then 2 + 2 (i - 2) + kk.
+// Block (i, kk) of a lower- or upper-triangular 64 x 64 operand (rows 16 i,
+// columns 32 kk) among its kTri stored ones, row by row.
 __device__ __forceinline__ constexpr int lower_block(int i, int kk) { return i < 2 ? i : 2 * (i - 1) + kk; }
-__device__ __forceinline__ constexpr int lower_steps(int i) { return i < 2 ? 1 : 2; }
+__device__ __forceinline__ constexpr int upper_block(int i, int kk) { return i < 2 ? 2 * i + kk : i + 2; }
 
-// What delta_prep leaves for a chunk of a head: row factors, then T and
-// scale (tril(Q K^T) . D) diag(beta) as operands, block by block, part by part,
-// sixteen bytes a lane.
-template <typename T> struct Record {
-    static constexpr int kK = 0, kQ = 64, kU = 128, kEnd = 192;    // floats: exp(G) rk, scale exp(G) rq,
+// What delta_prep leaves for a chunk of a head, in kilobytes: row factors, then
+// triangular operands block by block, part by part, sixteen bytes a lane.  The
+// window's kernel takes T and the attention scale (tril(Q K^T) . D) diag(beta);
+// the backward's T for the states on the way in and both transposed for the way
+// back.
+constexpr int kFacK = 0, kFacQ = 64, kFacU = 128, kFacEnd = 192;   // floats: exp(G) rk, scale exp(G) rq,
                                                                    // beta exp(G_C - G) rk, exp(G_C)
-    static constexpr size_t factors = 1024;
-    static constexpr size_t tri(int parts) { return size_t(kTri) * parts * 1024; }
-    static constexpr size_t t_at = factors, p_at = t_at + tri(kNP);
-    static constexpr size_t bytes = p_at + tri(Parts<T>::out);
+constexpr int kTriT = kTri * kNP;                                  // kilobytes of T
+template <typename T> struct Record {
+    static constexpr int t = 1, p = t + kTriT, units = p + kTri * Parts<T>::out;
 };
+struct BackRecord {
+    static constexpr int t = 1, tt = t + kTriT, pt = tt + kTriT, units = pt + kTriT;
+};
+
+// The fetch of a chunk's operands to LDS: K, Q if WITHQ, a 64-column tile of v
+// (or dy), and UNITS kilobytes of its record (unit u > 0 from kilobyte u + GAP).
+// bf16 with aligned rows (DMA): straight from memory, in four parts that the
+// caller spreads over its products.  Other inputs become their bf16 parts on
+// the way, through registers; v stays in registers.
+template <typename T, int N, bool VEC, bool WITHQ, int UNITS, int GAP>
+struct Stage {
+    static constexpr int KP = Parts<T>::in;
+    static constexpr bool DMA = VEC && std::is_same<T, bf16_t>::value;
+    static constexpr int pieces = kC * N / 8 / 256, rpieces = UNITS / 4 + 1;
+    struct Buf {
+        unsigned char k[KP][Tile<N>::bytes], q[WITHQ ? KP : 1][WITHQ ? Tile<N>::bytes : 16];
+        unsigned char v[DMA ? Tile<64>::bytes : 16];
+        unsigned char rec[UNITS * 1024];
+    };
+    const T *kp, *qp, *vp;              // the sequence's rows of this head
+    size_t ks, qs, vs, rec_bytes;
+    const unsigned char *rec;           // the sequence's records
+    int len, n_of, P, w, lane;
+    uint32_t dk, dq, dv;                // DMA places
+    int kt, kn, vt, vn;                 // else: this thread's places
+    uint32_t k_at, q_at, v_at;
+    Eight<T> k8[pieces], q8[WITHQ ? pieces : 1];
+    u32x4 r8[rpieces];
+    uint32_t v1[4][4];
+
+    __device__ __forceinline__ Stage(const DeltaLaunch &a, size_t b, size_t h, int length, const T *v, size_t vstride,
+                                     int p0, const unsigned char *records, size_t record_bytes) {
+        const int tid = threadIdx.x;
+        lane = tid & 63;
+        w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        len = length;
+        n_of = static_cast<int>(a.d_state);
+        P = static_cast<int>(a.head_dim);
+        const size_t kg = h / (a.heads / a.groups);
+        ks = a.ks;
+        qs = a.qs;
+        vs = vstride;
+        kp = static_cast<const T *>(a.k) + b * a.seq * ks + kg * n_of;
+        qp = static_cast<const T *>(a.q) + b * a.seq * qs + kg * n_of;
+        vp = v;
+        rec = records;
+        rec_bytes = record_bytes;
+        kt = tid / (N / 8);
+        kn = tid % (N / 8) * 8;
+        vt = 4 * (lane >> 4);
+        vn = p0 + 16 * w + (lane & 15);
+        if constexpr (DMA) {
+            dk = dma_at<T, N>(ks, n_of, 0, w, lane);
+            dq = dma_at<T, N>(qs, n_of, 0, w, lane);
+            dv = dma_at<T, 64>(vs, P, p0, w, lane);
+        } else {
+            k_at = row_off<T>(ks, n_of, kt, kn);
+            q_at = row_off<T>(qs, n_of, kt, kn);
+            v_at = row_off<T>(vs, P, vt, vn);
+        }
+    }
+    __device__ __forceinline__ rsrc_t record(int ck) const { return make_rsrc(rec + ck * rec_bytes, static_cast<uint32_t>(rec_bytes)); }
+    static __device__ __forceinline__ constexpr int unit(int u) { return u == 0 ? 0 : u + GAP; }
+
+    __device__ __forceinline__ void dma(Buf &to, int ck, int part) const {
+        const size_t t0 = static_cast<size_t>(ck) * kC;
+        const int left = len - ck * kC;
+        if (part == 0) dma_tile<N>(Rows<T, true>(kp + t0 * ks, ks, left, n_of), dk, to.k[0], w);
+        if (part == 1 && WITHQ) dma_tile<N>(Rows<T, true>(qp + t0 * qs, qs, left, n_of), dq, to.q[0], w);
+        if (part == 2) dma_tile<64>(Rows<T, true>(vp + t0 * vs, vs, left, P), dv, to.v, w);
+        if (part >= 2) {
+            const rsrc_t r = record(ck);
+            constexpr int half = (UNITS + 7) / 8;
+#pragma unroll
+            for (int i = 0; i < half; ++i) {
+                const int u = w + 4 * (i + (part - 2) * half);
+                if (u < UNITS) scan::lds_dma16(r, scan::lds_addr(to.rec + u * 1024), unit(u) * 1024 + lane * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void fetch(int ck) {
+        const size_t t0 = static_cast<size_t>(ck) * kC;
+        const int left = len - ck * kC;
+        const Rows<T, VEC> kr(kp + t0 * ks, ks, left, n_of), qr(qp + t0 * qs, qs, left, n_of);
+        const Rows<T, VEC> vr(vp + t0 * vs, vs, left, P);
+#pragma unroll
+        for (int i = 0; i < pieces; ++i) {
+            k8[i] = load_eight(kr, k_at, kt, kn, i * (2048 / N));
+            if constexpr (WITHQ) q8[i] = load_eight(qr, q_at, kt, kn, i * (2048 / N));
+        }
+        const rsrc_t r = record(ck);
+#pragma unroll
+        for (int i = 0; i < rpieces; ++i) r8[i] = bld16(r, unit(w + 4 * i) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r1 = 0; r1 < 4; ++r1) v1[i][r1] = load_one(vr, v_at, vt, vn, 16 * i + r1);
+    }
+    __device__ __forceinline__ void put(Buf &to) const {
+#pragma unroll
+        for (int i = 0; i < pieces; ++i) {
+            bf16x8 x[KP];
+            const int at = tile_at<N>(kt + i * (2048 / N), kn / 8);
+            to_parts(k8[i], x);
+#pragma unroll
+            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(to.k[q] + at) = x[q];
+            if constexpr (WITHQ) {
+                to_parts(q8[i], x);
+#pragma unroll
+                for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(to.q[q] + at) = x[q];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < rpieces; ++i)
+            if (w + 4 * i < UNITS) *reinterpret_cast<u32x4 *>(to.rec + (w + 4 * i) * 1024 + lane * 16) = r8[i];
+    }
+    // v as accumulator tiles
+    __device__ __forceinline__ void values(const Buf &from, f32x4 *e) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DMA) {
+                const bf16x4 x = tile_acc(from.v, i, w, lane);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) e[i][r] = static_cast<float>(x[r]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) e[i][r] = value_of<T>(v1[i][r]);
+            }
+        }
+    }
+};
+
+// Blocks of a lower (upper) triangle that take the first k-step, then those that
+// take the second, with the accumulator tile each adds to.
+template <int NP>
+__device__ __forceinline__ bf16x8 tri_block(const unsigned char *base, int blk, int q, int lane) {
+    return *reinterpret_cast<const bf16x8 *>(base + ((blk * NP + q) * 64 + lane) * 16);
+}
+template <int NP>
+__device__ __forceinline__ void tri_load(const unsigned char *base, int lane, bf16x8 (*all)[NP], bf16x8 (*part)[NP],
+                                         bool upper) {
+    // lower: block 0: (0, 0), 1: (1, 0), 2: (2, 0), 3: (2, 1), 4: (3, 0), 5: (3, 1)
+    // upper: 0: (0, 0), 1: (0, 1), 2: (1, 0), 3: (1, 1), 4: (2, 1), 5: (3, 1)
+    const int al[4] = {0, 1, 2, 4}, pl[2] = {3, 5}, au[4] = {1, 3, 4, 5}, pu[2] = {0, 2};
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all[i][q] = tri_block<NP>(base, upper ? au[i] : al[i], q, lane);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) part[i][q] = tri_block<NP>(base, upper ? pu[i] : pl[i], q, lane);
+    }
+}
+
+// The chunk kernels' launches for the other passes (delta_chunk.hip).
+bool rows_vec(const DeltaLaunch &a, size_t size);
+inline size_t chunks_of(const DeltaLaunch &a) { return (a.seq + kC - 1) / kC; }
+
+template <typename F>
+hipError_t by_state(size_t d_state, F f) {
+    if (d_state <= 64) return f(std::integral_constant<int, 64>{});
+    return f(std::integral_constant<int, 128>{});
+}
+
+// What the backward keeps of each chunk of a head, f32: the state before it and
+// the gradient of the state after it [P64][N] (P64: head_dim to the next multiple
+// of 64, N: 64 or 128), E and dR [64][P64].
+struct Kept {
+    size_t p64, n;
+    __host__ __device__ Kept(const DeltaLaunch &a) : p64((a.head_dim + 63) / 64 * 64), n(a.d_state <= 64 ? 64 : 128) {}
+    __host__ __device__ size_t s0() const { return 0; }
+    __host__ __device__ size_t s1() const { return p64 * n; }
+    __host__ __device__ size_t e() const { return 2 * p64 * n; }
+    __host__ __device__ size_t dr() const { return 2 * p64 * n + kC * p64; }
+    __host__ __device__ size_t floats() const { return 2 * p64 * (n + kC); }
+};
+
+// delta_prep and the forward states of the backward (delta_chunk.hip).
+hipError_t launch_delta_states(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s, int &launches);
 
 }  // namespace delta
 }  // namespace m3

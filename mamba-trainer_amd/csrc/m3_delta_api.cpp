@@ -130,7 +130,8 @@ m3_status m3_delta_step(const m3_delta_inputs *in, float *state, void *y, void *
 
 size_t m3_delta_rule_backward_workspace_bytes(const m3_delta_inputs *in) {
     if (check(in) != M3_OK) return 0;
-    return m3::delta_backward_workspace(launch_of(in));
+    const m3::DeltaLaunch a = launch_of(in);
+    return m3::delta_backward_supported(a) ? m3::delta_backward_workspace(a) : 0;
 }
 
 m3_status m3_delta_rule_backward(const m3_delta_inputs *in, const m3_delta_grads *gr, void *stream) {
@@ -143,8 +144,11 @@ m3_status m3_delta_rule_backward(const m3_delta_inputs *in, const m3_delta_grads
         return m3::api_fail(M3_ERR_ARGUMENT, "dy, dq, dk, dv, dg and dbeta are required");
     if ((in->state != nullptr) != (gr->dstate0 != nullptr))
         return m3::api_fail(M3_ERR_ARGUMENT, "dstate0 goes with the state before the window");
-    if (in->batch == 0) return m3::api_ok();
     const m3::DeltaLaunch a = launch_of(in);
+    if (!m3::delta_backward_supported(a))
+        return m3::api_fail(M3_ERR_UNSUPPORTED, "the delta rule's gradient takes d_state up to 128 (got %zu)",
+                            in->d_state);
+    if (in->batch == 0) return m3::api_ok();
     st = check_workspace(in, m3::delta_backward_workspace(a));
     if (st != M3_OK) return st;
     const m3::DeltaGrads g{gr->dy, gr->dstate, gr->dq, gr->dk, gr->dv, gr->dg, gr->dbeta, gr->dstate0};
