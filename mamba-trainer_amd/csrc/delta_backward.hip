@@ -201,26 +201,30 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
 }
 
 // One workgroup a (sequence, group, chunk), a wave sixteen of its tokens; the
-// heads that share the group's q and k in turn, their dq and dk summed in
-// registers.
-template <typename T, int N, bool VEC>
-__global__ void __launch_bounds__(256)
+// heads that share the group's q and k in turn.  First the triangles (F, Z, V and
+// the sums of V), then the products with the states, then those within the
+// chunk: what each holds in registers is gone before the next, so that two
+// workgroups fit a CU and one's loads pass behind the other's products.  MANY:
+// more than one head a group, whose dq and dk add up in further registers.
+template <typename T, int N, bool VEC, bool MANY>
+__global__ void __launch_bounds__(256, !MANY && Parts<T>::in == 1 ? 2 : 1)
 delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chunks, const float *kept) {
-    constexpr int KP = Parts<T>::in, OP = Parts<T>::out, NT = N / 16;
+    constexpr int KP = Parts<T>::in, OP = Parts<T>::out, NT = N / 16, per = N / 8;
     constexpr int s_bytes = kNP * Tile<N>::bytes / 2, xy_bytes = 2 * OP * Tile<64>::bytes, LW = kC + 1;
     constexpr int region = s_bytes > xy_bytes ? s_bytes : xy_bytes;
-    static_assert(region >= kC * LW * 4, "V shares the region");
+    static_assert(region >= kC * LW * 4 && region >= 2 * Tile<N>::bytes, "V and the outputs share the region");
     __shared__ __attribute__((aligned(16))) unsigned char sk[KP][Tile<N>::bytes], sq[KP][Tile<N>::bytes];
     __shared__ __attribute__((aligned(16))) unsigned char area[region];
-    __shared__ double G[kC];
-    __shared__ float beta[kC], rq[kC], rk[kC], da[kC], db[kC], dks[kC], dots[4];
+    __shared__ __attribute__((aligned(16))) float fac[256];
+    __shared__ double G[kC], sum_up[4][kC], sum_all[4][kC];
+    __shared__ float beta[kC], rq[kC], rk[kC], da[kC], db[kC], dots[4];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t id = blockIdx.x, ck = id % chunks, kg = id / chunks % a.groups, b = id / chunks / a.groups;
     const int L = static_cast<int>(a.seq), t0 = static_cast<int>(ck) * kC, left = L - t0;
     const int live = valid_len(a.lengths, b, L) - t0;
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
-    const size_t rep = a.heads / a.groups, qk = a.groups * n_of, out0 = (b * L + t0) * qk + kg * n_of;
+    const size_t rep = a.heads / a.groups, qk = a.groups * n_of, tok = b * L + t0, out0 = tok * qk + kg * n_of;
     T *dqp = static_cast<T *>(gr.dq) + out0, *dkp = static_cast<T *>(gr.dk) + out0;
     if (live <= 0) {   // padding: zeros
         const int rows = left < kC ? left : kC;
@@ -229,19 +233,19 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             stf(dkp + (i / n_of) * qk + i % n_of, 0.f);
         }
         for (int i = tid; i < rows * static_cast<int>(rep); i += 256) {
-            const size_t th = (b * L + t0 + i / rep) * a.heads + kg * rep + i % rep;
+            const size_t th = (tok + i / rep) * a.heads + kg * rep + i % rep;
             gr.dg[th] = gr.dbeta[th] = 0.f;
         }
         return;
     }
     const Kept kd(a);
+    const int my = 16 * w + c;
     // the group's rows, and the factors that bring them to unit length
     {
-        const Rows<T, VEC> kr(static_cast<const T *>(a.k) + (b * L + t0) * a.ks + kg * n_of, a.ks, live, n_of);
-        const Rows<T, VEC> qr(static_cast<const T *>(a.q) + (b * L + t0) * a.qs + kg * n_of, a.qs, live, n_of);
-        constexpr int per = N / 8;   // threads of a row
+        const Rows<T, VEC> kr(static_cast<const T *>(a.k) + tok * a.ks + kg * n_of, a.ks, live, n_of);
+        const Rows<T, VEC> qr(static_cast<const T *>(a.q) + tok * a.qs + kg * n_of, a.qs, live, n_of);
 #pragma unroll
-        for (int i = 0; i < kC * N / 8 / 256; ++i) {
+        for (int i = 0; i < kC * per / 256; ++i) {
             const int t = tid / per + i * (256 / per), n = tid % per * 8;
             const Eight<T> k8 = load_eight(kr, t, n), q8 = load_eight(qr, t, n);
             float f[8], ssk = 0.f, ssq = 0.f;
@@ -269,103 +273,134 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(sq[q] + tile_at<N>(t, n / 8)) = x[q];
         }
     }
-    __syncthreads();
-    f32x4 dq[NT], dk[NT], qkt[4], kkt[4];
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) dq[nt] = dk[nt] = zero;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) qkt[j] = kkt[j] = zero;
-#pragma unroll
-    for (int kk = 0; kk < N / 32; ++kk) {
-        bf16x8 qa[KP], ka[KP], kb[KP];
-#pragma unroll
-        for (int q = 0; q < KP; ++q) {
-            qa[q] = tile_rows<N>(sq[q], w, kk, lane);
-            ka[q] = tile_rows<N>(sk[q], w, kk, lane);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > w) continue;
-#pragma unroll
-            for (int q = 0; q < KP; ++q) kb[q] = tile_rows<N>(sk[q], j, kk, lane);
-            qkt[j] = mma_parts<KP, KP>(qa, kb, qkt[j]);
-            kkt[j] = mma_parts<KP, KP>(ka, kb, kkt[j]);
-        }
-    }
-    // q (or k) of this lane's place r of tile nt, from its parts
+    // q (or k) at row r, column state_n(nt, c >> 2, c & 3), from its parts
+    const int own = (16 * w + 4 * g) * (2 * N) + ((g ^ (c >> 2)) << 4) + 2 * (c & 3);
     const auto value = [&](const unsigned char(*t)[Tile<N>::bytes], int nt, int r) {
-        const int at = tile_at<N>(16 * w + 4 * g + r, 4 * (nt >> 1) + (c >> 2)) + 8 * (nt & 1) + 2 * (c & 3);
+        const int at = own + r * (2 * N) + (((nt >> 1) ^ (N == 128 ? r : r >> 1)) << 6) + 8 * (nt & 1);
         float v = 0.f;
 #pragma unroll
         for (int q = KP - 1; q >= 0; --q) v += bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(t[q] + at));
         return v;
     };
+    f32x4 dq[NT], dk[NT], tq[MANY ? NT : 1], tk[MANY ? NT : 1];
+    if constexpr (MANY)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) tq[nt] = tk[nt] = zero;
     for (size_t hr = 0; hr < rep; ++hr) {
         const size_t h = kg * rep + hr, rec = (b * a.heads + h) * chunks + ck;
-        const float *fac = reinterpret_cast<const float *>(records + rec * (BackRecord::units * 1024));
         const float *keep = kept + rec * kd.floats();
-        const Rows<T, VEC> dyr(static_cast<const T *>(gr.dy) + ((b * L + t0) * a.heads + h) * P, a.heads * P, live, P);
+        const Rows<T, VEC> dyr(static_cast<const T *>(gr.dy) + (tok * a.heads + h) * P, a.heads * P, live, P);
+        // rows of dY, dR, E: columns pb + 4g .. and pb + 16 + 4g ..
+        const auto kept_row = [&](size_t at, int t, int pb, bf16x8 *out) {
+            const float *s = keep + at + t * kd.p64 + pb + 4 * g;
+            split_tiles<kNP>(*reinterpret_cast<const f32x4 *>(s), *reinterpret_cast<const f32x4 *>(s + 16), out);
+        };
+        const auto dy_row = [&](int pb, bf16x8 *out) {
+            float y8[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
+                y8[j] = value_of<T>(load_one(dyr, row_off<T>(dyr.stride, P, my, n), my, n, 0));
+            }
+            split8<KP>(y8, out);
+        };
         if (w == 0) {
-            const size_t th = (b * L + t0 + lane) * a.heads + h;
+            const size_t th = (tok + lane) * a.heads + h;
             G[lane] = wave_scan<1>(lane < live ? static_cast<double>(clamp_decay(a.g[th])) : 0.0, lane);
             beta[lane] = lane < live ? a.beta[th] : 0.f;
         }
-        f32x4 qi[NT], ki[NT], ks[NT], f[4], z[4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) qi[nt] = ki[nt] = ks[nt] = zero;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = z[j] = zero;
-        float dot = 0.f;   // of S0 and dS1
+        if (w == 1)
+            *reinterpret_cast<f32x4 *>(fac + 4 * lane) =
+                *reinterpret_cast<const f32x4 *>(records + rec * (BackRecord::units * 1024) + 16 * lane);
+        f32x4 f[4] = {zero, zero, zero, zero}, z[4] = {zero, zero, zero, zero};
+#pragma unroll 1
         for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
-            constexpr int pieces = 32 * N / 8 / 256, per = N / 8;
-            const int pr = tid / per, pn = tid % per * 8;
-            float s0[pieces][8], s1[pieces][8];
-#pragma unroll
-            for (int i = 0; i < pieces; ++i) {
-                const float *s = keep + (pb + pr + i * (256 / per)) * N + pn;
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const f32x4 x0 = *reinterpret_cast<const f32x4 *>(s + kd.s0() + 4 * v);
-                    const f32x4 x1 = *reinterpret_cast<const f32x4 *>(s + kd.s1() + 4 * v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s0[i][4 * v + j] = x0[j];
-                        s1[i][4 * v + j] = x1[j];
-                        dot += x0[j] * x1[j];
-                    }
-                }
-            }
-            // rows of dY, dR, E: columns pb + 4g .. and pb + 16 + 4g ..
-            const auto kept_row = [&](size_t at, int t, bf16x8 *out) {
-                const float *s = keep + at + t * kd.p64 + pb + 4 * g;
-                split_tiles<kNP>(*reinterpret_cast<const f32x4 *>(s), *reinterpret_cast<const f32x4 *>(s + 16), out);
-            };
-            bf16x8 ya[KP], ra[kNP], ea[kNP];
-            {
-                float y8[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
-                    y8[j] = value_of<T>(load_one(dyr, row_off<T>(dyr.stride, P, 16 * w + c, n), 16 * w + c, n, 0));
-                }
-                split8<KP>(y8, ya);
-            }
-            kept_row(kd.dr(), 16 * w + c, ra);
-            kept_row(kd.e(), 16 * w + c, ea);
+            bf16x8 ya[KP], ra[kNP];
+            dy_row(pb, ya);
+            kept_row(kd.dr(), my, pb, ra);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j > w) continue;
                 bf16x8 eb[kNP];
-                kept_row(kd.e(), 16 * j + c, eb);
+                kept_row(kd.e(), 16 * j + c, pb, eb);
                 f[j] = mma_parts<KP, kNP>(ya, eb, f[j]);
                 z[j] = mma_parts<kNP, kNP>(ra, eb, z[j]);
             }
-            const auto put = [&](const float(*s)[8]) {
+        }
+        scan::lds_barrier();
+        {
+            f32x4 qkt[4] = {zero, zero, zero, zero}, kkt[4] = {zero, zero, zero, zero};
+#pragma unroll 1
+            for (int kk = 0; kk < N / 32; ++kk) {
+                bf16x8 qa[KP], ka[KP], kb[KP];
+#pragma unroll
+                for (int q = 0; q < KP; ++q) {
+                    qa[q] = tile_rows<N>(sq[q], w, kk, lane);
+                    ka[q] = tile_rows<N>(sk[q], w, kk, lane);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j > w) continue;
+#pragma unroll
+                    for (int q = 0; q < KP; ++q) kb[q] = tile_rows<N>(sk[q], j, kk, lane);
+                    qkt[j] = mma_parts<KP, KP>(qa, kb, qkt[j]);
+                    kkt[j] = mma_parts<KP, KP>(ka, kb, kkt[j]);
+                }
+            }
+            float(*V)[LW] = reinterpret_cast<float(*)[LW]>(area);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * w + 4 * g + r, jj = 16 * j + c;
+                    float x = 0.f, y = 0.f, v = 0.f;
+                    if (j <= w && jj <= i) {
+                        const float d = expf(static_cast<float>(G[i] - G[jj])) * rk[jj];
+                        x = a.scale * rq[i] * d * f[j][r];
+                        if (jj < i) y = rk[i] * d * z[j][r];
+                        v = x * qkt[j][r] - y * kkt[j][r];
+                    }
+                    V[i][jj] = v;
+                    f[j][r] = x * beta[jj];
+                    z[j][r] = -y * beta[jj];
+                }
+            scan::lds_barrier();
+            // each wave's rows (columns) of every token's sums
+            const int t = lane;
+            double col = 0.0, all = 0.0, across = 0.0;
+#pragma unroll 4
+            for (int n = 0; n < 16; ++n) {
+                const int i = 16 * w + n;
+                const double v = V[i][t];
+                if (i > t) col += v;
+                if (i >= t) all += v;
+                if (i < t) across += static_cast<double>(beta[i]) * V[t][i];
+            }
+            sum_up[w][t] = across - beta[t] * col;
+            sum_all[w][t] = all;
+        }
+        f32x4 ki[NT], dot4 = zero;   // dq: dY S0, ki: dR S0, dk: E dS1
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) dq[nt] = ki[nt] = dk[nt] = zero;
+#pragma unroll 1
+        for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
+            constexpr int pieces = 32 * N / 8 / 256;
+            const int pr = tid / per, pn = tid % per * 8;
+            f32x4 s0[pieces][2], s1[pieces][2];
+            const auto load = [&](size_t at, f32x4(*out)[2]) {
+#pragma unroll
+                for (int i = 0; i < pieces; ++i) {
+                    const float *s = keep + at + (pb + pr + i * (256 / per)) * N + pn;
+                    out[i][0] = *reinterpret_cast<const f32x4 *>(s);
+                    out[i][1] = *reinterpret_cast<const f32x4 *>(s + 4);
+                }
+            };
+            const auto put = [&](const f32x4(*s)[2]) {
 #pragma unroll
                 for (int i = 0; i < pieces; ++i) {
                     bf16x8 x[kNP];
-                    split8<kNP>(s[i], x);
+                    split_tiles<kNP>(s[i][0], s[i][1], x);
 #pragma unroll
                     for (int q = 0; q < kNP; ++q)
                         *reinterpret_cast<bf16x8 *>(area + q * (Tile<N>::bytes / 2) +
@@ -376,92 +411,61 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
 #pragma unroll
                 for (int q = 0; q < kNP; ++q) out[q] = tile_cols<N>(area + q * (Tile<N>::bytes / 2), nt, 0, lane);
             };
-            __syncthreads();
+            load(kd.s0(), s0);
+            load(kd.s1(), s1);
+            bf16x8 ya[KP], ra[kNP];
+            dy_row(pb, ya);
+            kept_row(kd.dr(), my, pb, ra);
+            scan::lds_barrier();
             put(s0);
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < pieces; ++i) dot4 += s0[i][0] * s1[i][0] + s0[i][1] * s1[i][1];
+            scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 bf16x8 s[kNP];
                 state(nt, s);
-                qi[nt] = mma_parts<KP, kNP>(ya, s, qi[nt]);
+                dq[nt] = mma_parts<KP, kNP>(ya, s, dq[nt]);
                 ki[nt] = mma_parts<kNP, kNP>(ra, s, ki[nt]);
+                if (nt & 1) __builtin_amdgcn_sched_barrier(0);
             }
-            __syncthreads();
+            kept_row(kd.e(), my, pb, ra);
+            scan::lds_barrier();
             put(s1);
-            __syncthreads();
+            scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 bf16x8 s[kNP];
                 state(nt, s);
-                ks[nt] = mma_parts<kNP, kNP>(ea, s, ks[nt]);
+                dk[nt] = mma_parts<kNP, kNP>(ra, s, dk[nt]);
+                if (nt & 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        dot = group_sum(dot, 64);
+        const float dot = group_sum(dot4[0] + dot4[1] + dot4[2] + dot4[3], 64);
         if (lane == 0) dots[w] = dot;
         // row by row: what the states contribute
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int t = 16 * w + 4 * g + r;
             const float fq = fac[kFacQ + t], fk = fac[kFacK + t], fu = fac[kFacU + t];
-            float xq = 0.f, xk = 0.f, xs = 0.f;
+            float x = 0.f, xs = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float kv = value(sk, nt, r);
-                xq += value(sq, nt, r) * qi[nt][r];
-                xk += kv * ki[nt][r];
-                xs += kv * ks[nt][r];
-                dq[nt][r] += fq * qi[nt][r];
-                dk[nt][r] += fu * ks[nt][r] - fk * ki[nt][r];
+                const float kv = value(sk, nt, r), ka = fk * ki[nt][r];
+                dq[nt][r] *= fq;
+                x += value(sq, nt, r) * dq[nt][r] - kv * ka;
+                xs += kv * dk[nt][r];
+                dk[nt][r] = fu * dk[nt][r] - ka;
             }
-            xq = row16(xq);
-            xk = row16(xk);
+            x = row16(x);
             xs = row16(xs);
             if (c == 0) {
-                da[t] = fq * xq - fk * xk;
-                db[t] = fu * xs;
-                dks[t] = rk[t] * xs;
+                da[t] = x;
+                db[t] = xs;
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // the triangle
-        __syncthreads();
-        float(*V)[LW] = reinterpret_cast<float(*)[LW]>(area);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * w + 4 * g + r, jj = 16 * j + c;
-                float x = 0.f, y = 0.f, v = 0.f;
-                if (jj <= i) {
-                    const float d = expf(static_cast<float>(G[i] - G[jj])) * rk[jj];
-                    x = a.scale * rq[i] * d * f[j][r];
-                    if (jj < i) y = rk[i] * d * z[j][r];
-                    v = x * qkt[j][r] - y * kkt[j][r];
-                }
-                V[i][jj] = v;
-                f[j][r] = x * beta[jj];
-                z[j][r] = -y * beta[jj];
-            }
-        __syncthreads();
-        if (w == 0) {
-            const int t = lane;
-            double col = 0.0, all = 0.0, row = 0.0;
-            for (int i = 0; i < kC; ++i) {
-                const double v = V[i][t];
-                if (i > t) col += v;
-                if (i >= t) all += v;
-                if (i < t) row += static_cast<double>(beta[i]) * V[t][i];
-            }
-            const double up = wave_scan<-1>(row - beta[t] * col + da[t], lane);
-            const double down = wave_scan<1>(db[t], lane) - db[t];
-            const float dot_all = dots[0] + dots[1] + dots[2] + dots[3];
-            const size_t th = (b * L + t0 + t) * a.heads + h;
-            if (t < left) {
-                const bool ok = t < live;
-                gr.dg[th] = ok ? static_cast<float>(up + down + static_cast<double>(fac[kFacEnd]) * dot_all) : 0.f;
-                gr.dbeta[th] = ok ? static_cast<float>(all + expf(static_cast<float>(G[kC - 1] - G[t])) * dks[t]) : 0.f;
-            }
-        }
-        __syncthreads();
+        scan::lds_barrier();
         // X and -Y as parts, then the products within the chunk
         const auto place = [&](int which, int q) { return area + (which * OP + q) * Tile<64>::bytes; };
 #pragma unroll
@@ -480,16 +484,29 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                     y -= to_f32(yb);
                 }
             }
-        __syncthreads();
-#pragma unroll
+        if (w == 0) {
+            const int t = lane;
+            const double up = wave_scan<-1>(sum_up[0][t] + sum_up[1][t] + sum_up[2][t] + sum_up[3][t] + da[t], lane);
+            const double all = sum_all[0][t] + sum_all[1][t] + sum_all[2][t] + sum_all[3][t];
+            const double bt = fac[kFacU + t] * db[t], down = wave_scan<1>(bt, lane) - bt;
+            const float dot_all = dots[0] + dots[1] + dots[2] + dots[3];
+            const size_t th = (tok + t) * a.heads + h;
+            if (t < left) {
+                const bool ok = t < live;
+                gr.dg[th] = ok ? static_cast<float>(up + down + static_cast<double>(fac[kFacEnd]) * dot_all) : 0.f;
+                gr.dbeta[th] = ok ? static_cast<float>(all + expf(static_cast<float>(G[kC - 1] - G[t])) * rk[t] * db[t]) : 0.f;
+            }
+        }
+        scan::lds_barrier();
+#pragma unroll 1
         for (int kk = 0; kk < 2; ++kk) {
             // rows 16 w of X and Y (tokens 32 kk + 4g .., + 16 + 4g ..), and of their transposes
             bf16x8 xr[OP], yr[OP], xt[OP], yt[OP];
 #pragma unroll
             for (int q = 0; q < OP; ++q) {
-                const int piece = 4 * kk + (g >> 1), off = 8 * (g & 1), t = 16 * w + c;
+                const int piece = 4 * kk + (g >> 1), off = 8 * (g & 1);
                 const auto four = [&](int which, int pc) {
-                    return *reinterpret_cast<const bf16x4 *>(place(which, q) + tile_at<64>(t, pc) + off);
+                    return *reinterpret_cast<const bf16x4 *>(place(which, q) + tile_at<64>(my, pc) + off);
                 };
                 xr[q] = __builtin_shufflevector(four(0, piece), four(0, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
                 yr[q] = __builtin_shufflevector(four(1, piece), four(1, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
@@ -513,10 +530,23 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                     dk[nt] = mma_parts<OP, KP>(xt, qc, dk[nt]);
                     dk[nt] = mma_parts<OP, KP>(yt, kc, dk[nt]);
                 }
+                if (nt & 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __syncthreads();
+        scan::lds_barrier();
+        if constexpr (MANY)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                tq[nt] += dq[nt];
+                tk[nt] += dk[nt];
+            }
     }
+    if constexpr (MANY)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            dq[nt] = tq[nt];
+            dk[nt] = tk[nt];
+        }
     // through the norm, and out
     const Rows<T, VEC> dqr(dqp, qk, left, n_of), dkr(dkp, qk, left, n_of);
 #pragma unroll
@@ -535,9 +565,28 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int n = state_n(nt, c >> 2, c & 3);
+            const float q = dq[nt][r] - value(sq, nt, r) * xq, k = dk[nt][r] - value(sk, nt, r) * xk;
+            if constexpr (VEC && sizeof(T) == 2) {
+                T *at = reinterpret_cast<T *>(area + tile_at<N>(t, n / 8) + 2 * (n % 8));
+                stf(at, q);
+                stf(at + Tile<N>::bytes / 2, k);
+            } else {
+                const uint32_t at = row_off<T>(qk, n_of, t, n);
+                store_one(dqr, at, t, n, 0, q);
+                store_one(dkr, at, t, n, 0, k);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (VEC && sizeof(T) == 2) {
+        scan::lds_barrier();
+#pragma unroll
+        for (int i = 0; i < kC * per / 256; ++i) {
+            const int t = tid / per + i * (256 / per), n = tid % per * 8;
             const uint32_t at = row_off<T>(qk, n_of, t, n);
-            store_one(dqr, at, t, n, 0, dq[nt][r] - value(sq, nt, r) * xq);
-            store_one(dkr, at, t, n, 0, dk[nt][r] - value(sk, nt, r) * xk);
+            const unsigned char *s = area + tile_at<N>(t, n / 8);
+            bst16(*reinterpret_cast<const u32x4 *>(s), dqr.r, at);
+            bst16(*reinterpret_cast<const u32x4 *>(s + Tile<N>::bytes), dkr.r, at);
         }
     }
 }
@@ -576,7 +625,10 @@ hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void
                 hipLaunchKernelGGL((delta_reverse<T, N, VEC>), rev, dim3(256), 0, s, a, g, records, chunks, kept);
                 ++launches;
                 if (chunks > 0) {
-                    hipLaunchKernelGGL((delta_grads<T, N, VEC>), own, dim3(256), 0, s, a, g, records, chunks, kept);
+                    if (a.heads == a.groups)
+                        hipLaunchKernelGGL((delta_grads<T, N, VEC, false>), own, dim3(256), 0, s, a, g, records, chunks, kept);
+                    else
+                        hipLaunchKernelGGL((delta_grads<T, N, VEC, true>), own, dim3(256), 0, s, a, g, records, chunks, kept);
                     ++launches;
                 }
                 return hipGetLastError();
