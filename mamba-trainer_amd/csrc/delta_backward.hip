@@ -287,22 +287,27 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
     if constexpr (MANY)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) tq[nt] = tk[nt] = zero;
-    for (size_t hr = 0; hr < rep; ++hr) {
+    for (size_t hr = 0; hr < (MANY ? rep : 1); ++hr) {
         const size_t h = kg * rep + hr, rec = (b * a.heads + h) * chunks + ck;
         const float *keep = kept + rec * kd.floats();
         const Rows<T, VEC> dyr(static_cast<const T *>(gr.dy) + (tok * a.heads + h) * P, a.heads * P, live, P);
-        // rows of dY, dR, E: columns pb + 4g .. and pb + 16 + 4g ..
-        const auto kept_row = [&](size_t at, int t, int pb, bf16x8 *out) {
+        // rows of dY, dR, E as loaded: columns pb + 4g .. and pb + 16 + 4g ..
+        const auto kept_row = [&](size_t at, int t, int pb, f32x4 *out) {
             const float *s = keep + at + t * kd.p64 + pb + 4 * g;
-            split_tiles<kNP>(*reinterpret_cast<const f32x4 *>(s), *reinterpret_cast<const f32x4 *>(s + 16), out);
+            out[0] = *reinterpret_cast<const f32x4 *>(s);
+            out[1] = *reinterpret_cast<const f32x4 *>(s + 16);
         };
-        const auto dy_row = [&](int pb, bf16x8 *out) {
-            float y8[8];
+        const auto dy_row = [&](int pb, uint32_t *out) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
-                y8[j] = value_of<T>(load_one(dyr, row_off<T>(dyr.stride, P, my, n), my, n, 0));
+                out[j] = load_one(dyr, row_off<T>(dyr.stride, P, my, n), my, n, 0);
             }
+        };
+        const auto dy_parts = [&](const uint32_t *y, bf16x8 *out) {
+            float y8[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y8[j] = value_of<T>(y[j]);
             split8<KP>(y8, out);
         };
         if (w == 0) {
@@ -314,20 +319,58 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             *reinterpret_cast<f32x4 *>(fac + 4 * lane) =
                 *reinterpret_cast<const f32x4 *>(records + rec * (BackRecord::units * 1024) + 16 * lane);
         f32x4 f[4] = {zero, zero, zero, zero}, z[4] = {zero, zero, zero, zero};
-#pragma unroll 1
-        for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
-            bf16x8 ya[KP], ra[kNP];
-            dy_row(pb, ya);
-            kept_row(kd.dr(), my, pb, ra);
+        {
+            uint32_t y1[8];
+            f32x4 r1[2], e1[4][2];
+            const auto load = [&](int pb) {
+                dy_row(pb, y1);
+                kept_row(kd.dr(), my, pb, r1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j > w) continue;
-                bf16x8 eb[kNP];
-                kept_row(kd.e(), 16 * j + c, pb, eb);
-                f[j] = mma_parts<KP, kNP>(ya, eb, f[j]);
-                z[j] = mma_parts<kNP, kNP>(ra, eb, z[j]);
+                for (int j = 0; j < 4; ++j)
+                    if (j <= w) kept_row(kd.e(), 16 * j + c, pb, e1[j]);
+            };
+            load(0);
+#pragma unroll 1
+            for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
+                bf16x8 ya[KP], ra[kNP], eb[4][kNP];
+                dy_parts(y1, ya);
+                split_tiles<kNP>(r1[0], r1[1], ra);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j <= w) split_tiles<kNP>(e1[j][0], e1[j][1], eb[j]);
+                if (pb + 32 < static_cast<int>(kd.p64)) load(pb + 32);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j > w) continue;
+                    f[j] = mma_parts<KP, kNP>(ya, eb[j], f[j]);
+                    z[j] = mma_parts<kNP, kNP>(ra, eb[j], z[j]);
+                }
             }
         }
+        // what the states' first block takes, on its way during the triangle
+        constexpr int pieces = 32 * N / 8 / 256;
+        const int pr = tid / per, pn = tid % per * 8;
+        f32x4 s0[pieces][2], s1[pieces][2], r1[2], e1[2];
+        uint32_t y1[8];
+        const auto load_state = [&](size_t at, int pb, f32x4(*out)[2]) {
+#pragma unroll
+            for (int i = 0; i < pieces; ++i) {
+                const float *s = keep + at + (pb + pr + i * (256 / per)) * N + pn;
+                out[i][0] = *reinterpret_cast<const f32x4 *>(s);
+                out[i][1] = *reinterpret_cast<const f32x4 *>(s + 4);
+            }
+        };
+        const auto load_first = [&](int pb) {
+            load_state(kd.s0(), pb, s0);
+            dy_row(pb, y1);
+            kept_row(kd.dr(), my, pb, r1);
+        };
+        const auto load_second = [&](int pb) {
+            load_state(kd.s1(), pb, s1);
+            kept_row(kd.e(), my, pb, e1);
+        };
+        load_first(0);
+        load_second(0);
         scan::lds_barrier();
         {
             f32x4 qkt[4] = {zero, zero, zero, zero}, kkt[4] = {zero, zero, zero, zero};
@@ -385,17 +428,6 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
         for (int nt = 0; nt < NT; ++nt) dq[nt] = ki[nt] = dk[nt] = zero;
 #pragma unroll 1
         for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
-            constexpr int pieces = 32 * N / 8 / 256;
-            const int pr = tid / per, pn = tid % per * 8;
-            f32x4 s0[pieces][2], s1[pieces][2];
-            const auto load = [&](size_t at, f32x4(*out)[2]) {
-#pragma unroll
-                for (int i = 0; i < pieces; ++i) {
-                    const float *s = keep + at + (pb + pr + i * (256 / per)) * N + pn;
-                    out[i][0] = *reinterpret_cast<const f32x4 *>(s);
-                    out[i][1] = *reinterpret_cast<const f32x4 *>(s + 4);
-                }
-            };
             const auto put = [&](const f32x4(*s)[2]) {
 #pragma unroll
                 for (int i = 0; i < pieces; ++i) {
@@ -411,15 +443,14 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
 #pragma unroll
                 for (int q = 0; q < kNP; ++q) out[q] = tile_cols<N>(area + q * (Tile<N>::bytes / 2), nt, 0, lane);
             };
-            load(kd.s0(), s0);
-            load(kd.s1(), s1);
             bf16x8 ya[KP], ra[kNP];
-            dy_row(pb, ya);
-            kept_row(kd.dr(), my, pb, ra);
+            dy_parts(y1, ya);
+            split_tiles<kNP>(r1[0], r1[1], ra);
             scan::lds_barrier();
             put(s0);
 #pragma unroll
             for (int i = 0; i < pieces; ++i) dot4 += s0[i][0] * s1[i][0] + s0[i][1] * s1[i][1];
+            if (pb + 32 < static_cast<int>(kd.p64)) load_first(pb + 32);
             scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -429,9 +460,10 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                 ki[nt] = mma_parts<kNP, kNP>(ra, s, ki[nt]);
                 if (nt & 1) __builtin_amdgcn_sched_barrier(0);
             }
-            kept_row(kd.e(), my, pb, ra);
+            split_tiles<kNP>(e1[0], e1[1], ra);
             scan::lds_barrier();
             put(s1);
+            if (pb + 32 < static_cast<int>(kd.p64)) load_second(pb + 32);
             scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
