@@ -15,6 +15,7 @@
 // contiguous.
 #include "delta.hpp"
 #include "m3_internal.hpp"
+#include "scan_common.hpp"
 
 namespace m3 {
 namespace {
@@ -23,17 +24,9 @@ using namespace delta;
 
 constexpr int E = 8;
 
-template <typename T> struct Raw8 {
-    uint4 q;
-    __device__ __forceinline__ void ld(const T *p) { q = *reinterpret_cast<const uint4 *>(p); }
-};
-template <> struct Raw8<float> {
-    f32x4 a, b;
-    __device__ __forceinline__ void ld(const float *p) {
-        a = *reinterpret_cast<const f32x4 *>(p);
-        b = *reinterpret_cast<const f32x4 *>(p + 4);
-    }
-};
+// Eight values as loaded.
+template <typename T> struct Raw8 { u32x4 q; };
+template <> struct Raw8<float> { f32x4 a, b; };
 __device__ __forceinline__ void wide(const Raw8<float> &r, float *f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -42,19 +35,17 @@ __device__ __forceinline__ void wide(const Raw8<float> &r, float *f) {
     }
 }
 __device__ __forceinline__ void wide(const Raw8<bf16_t> &r, float *f) {
-    const uint32_t u[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(u[i] << 16);
-        f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        f[2 * i] = __uint_as_float(r.q[i] << 16);
+        f[2 * i + 1] = __uint_as_float(r.q[i] & 0xFFFF0000u);
     }
 }
 __device__ __forceinline__ void wide(const Raw8<f16_t> &r, float *f) {
-    const uint32_t u[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u[i])));
-        f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u[i] >> 16)));
+        f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.q[i])));
+        f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.q[i] >> 16)));
     }
 }
 __device__ __forceinline__ void store8(float *p, const float *f) {
@@ -79,24 +70,50 @@ template <bool VEC, int NT>
 __device__ __forceinline__ int at(int tid, int c, int e) {
     return VEC ? (c * NT + tid) * E + e : (c * E + e) * NT + tid;
 }
+// Without a branch where the loads are whole pieces: a thread past the row reads
+// its start, and `wide_row` puts zeros there.
 template <bool VEC, int NT, typename T>
-__device__ __forceinline__ void load(const T *row, int tid, int c, int dim, float pad, float *f) {
+__device__ __forceinline__ Raw8<T> load_raw(const T *row, int tid, int c, int dim) {
+    Raw8<T> r;
     if constexpr (VEC) {
-        const int i = at<true, NT>(tid, c, 0);
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = pad;
-        if (i < dim) {
-            Raw8<T> r;
-            r.ld(row + i);
-            wide(r, f);
+        const int i = at<true, NT>(tid, c, 0), k = i < dim ? i : 0;
+        if constexpr (sizeof(T) == 4) {
+            r.a = *reinterpret_cast<const f32x4 *>(row + k);
+            r.b = *reinterpret_cast<const f32x4 *>(row + k + 4);
+        } else {
+            r.q = *reinterpret_cast<const u32x4 *>(row + k);
         }
     } else {
+        uint32_t u[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = at<false, NT>(tid, c, e);
-            f[e] = i < dim ? ldf(row + i) : pad;
+            const T x = row[i < dim ? i : 0];
+            u[e] = sizeof(T) == 4 ? __builtin_bit_cast(uint32_t, ldf(&x)) : *reinterpret_cast<const uint16_t *>(&x);
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                r.a[e] = __uint_as_float(u[e]);
+                r.b[e] = __uint_as_float(u[4 + e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.q[e] = u[2 * e] | u[2 * e + 1] << 16;
         }
     }
+    return r;
+}
+template <bool VEC, int NT, typename T>
+__device__ __forceinline__ void wide_row(const Raw8<T> &r, int tid, int c, int dim, float *f) {
+    wide(r, f);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (at<VEC, NT>(tid, c, e) >= dim) f[e] = 0.f;
+}
+template <bool VEC, int NT, typename T>
+__device__ __forceinline__ void load(const T *row, int tid, int c, int dim, float *f) {
+    wide_row<VEC, NT>(load_raw<VEC, NT>(row, tid, c, dim), tid, c, dim, f);
 }
 template <bool VEC, int NT, typename T>
 __device__ __forceinline__ void store(T *row, int tid, int c, int dim, const float *f) {
@@ -112,31 +129,35 @@ __device__ __forceinline__ void store(T *row, int tid, int c, int dim, const flo
     }
 }
 
-// act(z) and, with D, its derivative.
+// act(z) and its derivative, from one exponential and one reciprocal (v_rcp_f32,
+// within one unit in the last place).
 enum { kNone = 0, kSilu = 1, kSigmoid = 2 };
-__device__ __forceinline__ float act_of(int act, float z) {
-    if (act == kNone) return z;
-    const float s = 1.0f / (1.0f + expf(-z));
-    return act == kSilu ? z * s : s;
-}
-__device__ __forceinline__ float dact_of(int act, float z) {
-    if (act == kNone) return 1.0f;
-    const float s = 1.0f / (1.0f + expf(-z));
-    return act == kSilu ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+__device__ __forceinline__ float act_of(int act, float z, float &d) {
+    if (act == kNone) {
+        d = 1.0f;
+        return z;
+    }
+    const float s = __builtin_amdgcn_rcpf(1.0f + expf(-z));
+    if (act == kSigmoid) {
+        d = s * (1.0f - s);
+        return s;
+    }
+    d = s * (1.0f + z * (1.0f - s));
+    return z * s;
 }
 
-// Sums of K values over the NT threads of a row; `red` is this row's own
-// [K][NT / 64] and used once per call site.
+// Sums of K values over the NT threads of a row; `red` is [K][NT / 64], its
+// own for each call site, so that one barrier a sum is enough as long as
+// another call's stands between two uses.  Loads on their way stay so.
 template <int NT, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float *red, int tid) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = group_sum(v[k], 64);
+    for (int k = 0; k < K; ++k) v[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(seg_scan<64>(v[k])), 63));
     if constexpr (NT > 64) {
-        __syncthreads();
         if ((tid & 63) == 0)
 #pragma unroll
             for (int k = 0; k < K; ++k) red[k * (NT / 64) + (tid >> 6)] = v[k];
-        __syncthreads();
+        scan::lds_barrier();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float s = 0.f;
@@ -152,26 +173,26 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float *red, int tid) {
 template <typename T, typename RT, int NT, int NC, bool VEC>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNormLaunch a) {
     constexpr int RPW = NT < 256 ? 256 / NT : 1;
-    __shared__ float red[NT > 64 ? RPW * (NT / 64) : 1];
+    __shared__ float red[2][NT / 64];   // a row of more than a wave is the workgroup's
     const int tid = threadIdx.x % NT, sub = threadIdx.x / NT;
     const size_t row = static_cast<size_t>(blockIdx.x) * RPW + sub;
-    const bool live = row < a.rows;   // every thread meets the barriers
-    const int dim = live ? static_cast<int>(a.dim) : 0;
+    if (RPW > 1 && row >= a.rows) return;   // no barrier there
+    const int dim = static_cast<int>(a.dim);
     const float inv = 1.0f / static_cast<float>(a.dim);
     float x[NC][E], r[NC][E];
     float sx[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        load<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim, 0.f, x[c]);
+        load<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim, x[c]);
 #pragma unroll
         for (int e = 0; e < E; ++e) sx[0] += x[c][e] * x[c][e];
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-        load<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim, 0.f, r[c]);
+        load<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim, r[c]);
     float rx = 1.0f;
     if (a.post_norm) {
-        row_sum<NT>(sx, red + sub * (NT / 64), tid);
+        row_sum<NT>(sx, red[0], tid);
         rx = 1.0f / sqrtf(sx[0] * inv + a.eps);
     }
     float sr[1] = {0.f};
@@ -181,17 +202,18 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
 #pragma unroll
         for (int e = 0; e < E; ++e) x[c][e] *= rx;
         if (a.post_w) {
-            load<VEC, NT>(a.post_w, tid, c, dim, 0.f, f);
+            load<VEC, NT>(a.post_w, tid, c, dim, f);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[c][e] *= f[e];
         }
         if (a.gate) {
-            load<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim, 0.f, f);
+            load<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim, f);
+            float unused;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[c][e] *= act_of(a.act, f[e]);
+            for (int e = 0; e < E; ++e) x[c][e] *= act_of(a.act, f[e], unused);
         }
         if (a.scale) {
-            load<VEC, NT>(a.scale, tid, c, dim, 0.f, f);
+            load<VEC, NT>(a.scale, tid, c, dim, f);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[c][e] *= f[e];
         }
@@ -203,7 +225,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
         store<VEC, NT>(static_cast<RT *>(a.residual_out) + row * a.dim, tid, c, dim, r[c]);
     }
     if (a.y == nullptr) return;
-    row_sum<NT>(sr, red + sub * (NT / 64), tid);
+    row_sum<NT>(sr, red[1], tid);
     const float rho = 1.0f / sqrtf(sr[0] * inv + a.eps);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -211,7 +233,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
         for (int e = 0; e < E; ++e) r[c][e] *= rho;
         if (a.pre_w) {
             float f[E];
-            load<VEC, NT>(a.pre_w, tid, c, dim, 0.f, f);
+            load<VEC, NT>(a.pre_w, tid, c, dim, f);
 #pragma unroll
             for (int e = 0; e < E; ++e) r[c][e] *= f[e];
         }
@@ -219,94 +241,109 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
     }
 }
 
-// Gradients.  Workgroup i takes rows i, i + grid, ...; the column sums of the
-// three weights stay in its registers and go to partials[i][3][dim] at the end.
+// Gradients.  Workgroup i takes rows i, i + grid, ..., the next one's loads on
+// their way during this one's sums; the weights and the column sums of their
+// gradients stay in its registers (the sums go to partials[i][3][dim] at the
+// end).
 template <typename T, typename RT, int NT, int NC, bool VEC>
 __global__ void __launch_bounds__(NT) block_norm_backward_kernel(BlockNormLaunch a, BlockNormGrads g, float *partials) {
-    __shared__ float red[2 * (NT / 64)];
+    __shared__ float red[4][NT / 64];
     const int tid = threadIdx.x, dim = static_cast<int>(a.dim);
     const float inv = 1.0f / static_cast<float>(a.dim);
-    float spost[NC][E], sscale[NC][E], spre[NC][E];
+    float spost[NC][E], sscale[NC][E], spre[NC][E], w[NC][E], sc[NC][E], pw[NC][E];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) spost[c][e] = sscale[c][e] = spre[c][e] = 0.f;
+        for (int e = 0; e < E; ++e) {
+            spost[c][e] = sscale[c][e] = spre[c][e] = 0.f;
+            w[c][e] = sc[c][e] = pw[c][e] = 1.f;
+        }
+        if (a.post_w) load<VEC, NT>(a.post_w, tid, c, dim, w[c]);
+        if (a.scale) load<VEC, NT>(a.scale, tid, c, dim, sc[c]);
+        if (a.pre_w) load<VEC, NT>(a.pre_w, tid, c, dim, pw[c]);
+    }
+    Raw8<T> rx8[NC], rz8[NC], ry8[NC];
+    Raw8<RT> rr8[NC], rd8[NC];
+    const auto fetch = [&](size_t row) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            rx8[c] = load_raw<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim);
+            rr8[c] = load_raw<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim);
+            if (a.gate) rz8[c] = load_raw<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim);
+            if (g.dy) ry8[c] = load_raw<VEC, NT>(static_cast<const T *>(g.dy) + row * a.dim, tid, c, dim);
+            if (g.dres) rd8[c] = load_raw<VEC, NT>(static_cast<const RT *>(g.dres) + row * a.dim, tid, c, dim);
+        }
+    };
+    if (blockIdx.x < a.rows) fetch(blockIdx.x);
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float x[NC][E], r[NC][E], z[NC][E], dy[NC][E];
+        float x[NC][E], r[NC][E], dy[NC][E], d[NC][E];
+        float av[NC][E], dav[NC][E];   // the gate and its derivative
         float s1[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            load<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim, 0.f, x[c]);
-            load<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim, 0.f, r[c]);
-            if (a.gate) load<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim, 0.f, z[c]);
-            if (g.dy) load<VEC, NT>(static_cast<const T *>(g.dy) + row * a.dim, tid, c, dim, 0.f, dy[c]);
+            wide_row<VEC, NT>(rx8[c], tid, c, dim, x[c]);
+            wide_row<VEC, NT>(rr8[c], tid, c, dim, r[c]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                dy[c][e] = d[c][e] = dav[c][e] = 0.f;
+                av[c][e] = 1.f;
+            }
+            if (a.gate) {
+                float z[E];
+                wide_row<VEC, NT>(rz8[c], tid, c, dim, z);
+#pragma unroll
+                for (int e = 0; e < E; ++e) av[c][e] = act_of(a.act, z[e], dav[c][e]);
+            }
+            if (g.dy) wide_row<VEC, NT>(ry8[c], tid, c, dim, dy[c]);
+            if (g.dres) wide_row<VEC, NT>(rd8[c], tid, c, dim, d[c]);
 #pragma unroll
             for (int e = 0; e < E; ++e) s1[0] += x[c][e] * x[c][e];
         }
+        if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
         float rx = 1.0f;
         if (a.post_norm) {
-            row_sum<NT>(s1, red, tid);
+            row_sum<NT>(s1, red[0], tid);
             rx = 1.0f / sqrtf(s1[0] * inv + a.eps);
         }
         float s2[2] = {0.f, 0.f};
         float rho = 0.f, back = 0.f;
         if (g.dy) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float w[E], sc[E], pw[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) w[e] = sc[e] = pw[e] = 1.f;
-                if (a.post_w) load<VEC, NT>(a.post_w, tid, c, dim, 0.f, w);
-                if (a.scale) load<VEC, NT>(a.scale, tid, c, dim, 0.f, sc);
-                if (a.pre_w) load<VEC, NT>(a.pre_w, tid, c, dim, 0.f, pw);
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    r[c][e] += x[c][e] * rx * w[e] * (a.gate ? act_of(a.act, z[c][e]) : 1.f) * sc[e];
+                    r[c][e] += x[c][e] * rx * w[c][e] * av[c][e] * sc[c][e];
                     s2[0] += r[c][e] * r[c][e];
-                    s2[1] += dy[c][e] * pw[e] * r[c][e];
+                    s2[1] += dy[c][e] * pw[c][e] * r[c][e];
                 }
-            }
-            row_sum<NT>(s2, red, tid);
+            row_sum<NT>(s2, red[1], tid);
             rho = 1.0f / sqrtf(s2[0] * inv + a.eps);
             back = s2[1] * inv * rho * rho * rho;
         }
         float s3[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float d[E], w[E], sc[E], pw[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                w[e] = sc[e] = pw[e] = 1.f;
-                d[e] = 0.f;
-            }
-            if (g.dres) load<VEC, NT>(static_cast<const RT *>(g.dres) + row * a.dim, tid, c, dim, 0.f, d);
-            if (a.post_w) load<VEC, NT>(a.post_w, tid, c, dim, 0.f, w);
-            if (a.scale) load<VEC, NT>(a.scale, tid, c, dim, 0.f, sc);
-            if (a.pre_w) load<VEC, NT>(a.pre_w, tid, c, dim, 0.f, pw);
+            float dz[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 if (g.dy) {
                     spre[c][e] += dy[c][e] * r[c][e] * rho;
-                    d[e] += rho * dy[c][e] * pw[e] - r[c][e] * back;
+                    d[c][e] += rho * dy[c][e] * pw[c][e] - r[c][e] * back;
                 }
-            }
-            store<VEC, NT>(static_cast<RT *>(g.dresidual) + row * a.dim, tid, c, dim, d);
-            float dz[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float av = a.gate ? act_of(a.act, z[c][e]) : 1.f, n = x[c][e] * rx * w[e];
-                sscale[c][e] += av * n * d[e];
-                const float m = sc[e] * av * d[e];
-                dz[e] = a.gate ? sc[e] * n * d[e] * dact_of(a.act, z[c][e]) : 0.f;
+                const float n = x[c][e] * rx * w[c][e];
+                sscale[c][e] += av[c][e] * n * d[c][e];
+                const float m = sc[c][e] * av[c][e] * d[c][e];
+                dz[e] = sc[c][e] * n * d[c][e] * dav[c][e];
                 spost[c][e] += m * x[c][e] * rx;
-                r[c][e] = m * w[e];   // r is done with
+                r[c][e] = m * w[c][e];   // r is done with
                 s3[0] += r[c][e] * x[c][e];
             }
+            store<VEC, NT>(static_cast<RT *>(g.dresidual) + row * a.dim, tid, c, dim, d[c]);
             if (a.gate) store<VEC, NT>(static_cast<T *>(g.dgate) + row * a.dim, tid, c, dim, dz);
         }
         float mean = 0.f;
         if (a.post_norm) {
-            row_sum<NT>(s3, red, tid);
+            row_sum<NT>(s3, red[3], tid);
             mean = s3[0] * inv * rx * rx;
         }
 #pragma unroll
@@ -315,6 +352,8 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(BlockNormLaunch
             for (int e = 0; e < E; ++e) r[c][e] = rx * (r[c][e] - x[c][e] * mean);
             store<VEC, NT>(static_cast<T *>(g.dx) + row * a.dim, tid, c, dim, r[c]);
         }
+        // without a norm on either side of the add the loop has one sum or none
+        if (!(a.post_norm && g.dy)) scan::lds_barrier();
     }
     float *p = partials + static_cast<size_t>(blockIdx.x) * 3 * a.dim;
 #pragma unroll
@@ -325,22 +364,26 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(BlockNormLaunch
     }
 }
 
-// The partial sums of `parts` workgroups, in their order: one column a thread of
-// a row of 64, the parts dealt to four rows of threads.
-__global__ void __launch_bounds__(256) block_norm_columns(const float *partials, size_t parts, size_t dim, BlockNormGrads g) {
-    __shared__ float red[4][64];
-    const size_t col = blockIdx.x * size_t(64) + (threadIdx.x & 63);
-    const int q = threadIdx.x >> 6;
-    const size_t all = 3 * dim;
-    float s = 0.f;
-    if (col < all)
-        for (size_t i = q; i < parts; i += 4) s += partials[i * all + col];
-    red[q][threadIdx.x & 63] = s;
+// The partial sums of `parts` workgroups in a fixed order: 64 columns a
+// workgroup, the parts dealt to its 16 waves, eight on their way at once.
+__global__ void __launch_bounds__(1024) block_norm_columns(const float *partials, size_t parts, size_t dim, BlockNormGrads g) {
+    __shared__ float red[16][64];
+    const size_t all = 3 * dim, at = blockIdx.x * size_t(64) + (threadIdx.x & 63), col = at < all ? at : 0;
+    const size_t q = threadIdx.x >> 6;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    size_t i = q;
+    for (; i + 7 * 16 < parts; i += 8 * 16)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] += partials[(i + 16 * k) * all + col];
+    for (; i < parts; i += 16) s[0] += partials[i * all + col];
+    red[q][threadIdx.x & 63] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
-    if (q != 0 || col >= all) return;
-    s = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+    if (q != 0 || at >= all) return;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += red[k][threadIdx.x];
     float *out = col < dim ? g.dpost_w : col < 2 * dim ? g.dscale : g.dpre_w;
-    if (out) out[col % dim] = s;
+    if (out) out[col % dim] = t;
 }
 
 template <typename F>
@@ -424,11 +467,18 @@ hipError_t launch_block_norm_backward(const BlockNormLaunch &a, const BlockNormG
                                        s, a, g, partials);
                 return hipGetLastError();
             };
+            // one piece a thread as far as 2048 values: few enough registers for
+            // three waves a SIMD
+            using std::integral_constant;
+            constexpr integral_constant<int, 1> one{};
+            if (a.dim <= 512) return go(integral_constant<int, 64>{}, one);
+            if (a.dim <= 1024) return go(integral_constant<int, 128>{}, one);
+            if (a.dim <= 1536) return go(integral_constant<int, 192>{}, one);
             if (a.dim <= 8192) return by_pieces<256>(a.dim, go);
             return by_pieces<1024>(a.dim, go);
         });
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(block_norm_columns, dim3(static_cast<unsigned>((3 * a.dim + 63) / 64)), dim3(256), 0, s,
+    hipLaunchKernelGGL(block_norm_columns, dim3(static_cast<unsigned>((3 * a.dim + 63) / 64)), dim3(1024), 0, s,
                        partials, static_cast<size_t>(grid), a.dim, g);
     return hipGetLastError();
 }
