@@ -179,17 +179,27 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
     if (RPW > 1 && row >= a.rows) return;   // no barrier there
     const int dim = static_cast<int>(a.dim);
     const float inv = 1.0f / static_cast<float>(a.dim);
+    // every load of the row, and of the weights, on its way at once
+    Raw8<T> x8[NC], z8[NC];
+    Raw8<RT> r8[NC];
+    Raw8<float> w8[NC], s8[NC], p8[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        x8[c] = load_raw<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim);
+        r8[c] = load_raw<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim);
+        if (a.gate) z8[c] = load_raw<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim);
+        if (a.post_w) w8[c] = load_raw<VEC, NT>(a.post_w, tid, c, dim);
+        if (a.scale) s8[c] = load_raw<VEC, NT>(a.scale, tid, c, dim);
+        if (a.pre_w) p8[c] = load_raw<VEC, NT>(a.pre_w, tid, c, dim);
+    }
     float x[NC][E], r[NC][E];
     float sx[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        load<VEC, NT>(static_cast<const T *>(a.x) + row * a.dim, tid, c, dim, x[c]);
+        wide_row<VEC, NT>(x8[c], tid, c, dim, x[c]);
 #pragma unroll
         for (int e = 0; e < E; ++e) sx[0] += x[c][e] * x[c][e];
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-        load<VEC, NT>(static_cast<const RT *>(a.residual) + row * a.dim, tid, c, dim, r[c]);
     float rx = 1.0f;
     if (a.post_norm) {
         row_sum<NT>(sx, red[0], tid);
@@ -202,25 +212,26 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
 #pragma unroll
         for (int e = 0; e < E; ++e) x[c][e] *= rx;
         if (a.post_w) {
-            load<VEC, NT>(a.post_w, tid, c, dim, f);
+            wide(w8[c], f);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[c][e] *= f[e];
         }
         if (a.gate) {
-            load<VEC, NT>(static_cast<const T *>(a.gate) + row * a.gate_stride, tid, c, dim, f);
+            wide(z8[c], f);
             float unused;
 #pragma unroll
             for (int e = 0; e < E; ++e) x[c][e] *= act_of(a.act, f[e], unused);
         }
         if (a.scale) {
-            load<VEC, NT>(a.scale, tid, c, dim, f);
+            wide(s8[c], f);
 #pragma unroll
             for (int e = 0; e < E; ++e) x[c][e] *= f[e];
         }
+        wide(r8[c], r[c]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             r[c][e] += x[c][e];
-            sr[0] += r[c][e] * r[c][e];
+            sr[0] += at<VEC, NT>(tid, c, e) < dim ? r[c][e] * r[c][e] : 0.f;
         }
         store<VEC, NT>(static_cast<RT *>(a.residual_out) + row * a.dim, tid, c, dim, r[c]);
     }
@@ -233,7 +244,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) block_norm_kernel(BlockNo
         for (int e = 0; e < E; ++e) r[c][e] *= rho;
         if (a.pre_w) {
             float f[E];
-            load<VEC, NT>(a.pre_w, tid, c, dim, f);
+            wide(p8[c], f);
 #pragma unroll
             for (int e = 0; e < E; ++e) r[c][e] *= f[e];
         }
