@@ -203,65 +203,67 @@ _TYPES = {torch.float32: _lib.M3_F32, torch.bfloat16: _lib.M3_BF16, torch.float1
 _ACTIVATIONS = {"none": 0, "silu": 1, "sigmoid": 2}
 
 
-def _gate_rows(gate: torch.Tensor, shape) -> tuple:
+def _gate_rows(gate: torch.Tensor):
     """A gate read in place: (tensor, elements between its rows).  Rows that are
     evenly spaced and contiguous (columns of a projection) stay where they
     are; anything else is copied."""
-    if tuple(gate.shape) != tuple(shape):
-        raise ShapeError(f"shape error: gate has shape {list(gate.shape)}, expected {list(shape)}")
-    stride = gate.shape[-1]
-    ok = gate.stride(-1) == 1
-    if gate.dim() > 1:
-        stride = gate.stride(-2)
-        want = stride
-        for size, st in zip(reversed(gate.shape[:-1]), reversed(gate.stride()[:-1])):
-            ok = ok and (size == 1 or st == want)
-            want *= size
-    if gate.numel() > 0 and (not ok or stride < gate.shape[-1]):
-        gate = gate.contiguous()
-        stride = gate.shape[-1]
-    return gate, max(stride, gate.shape[-1])
+    dim = gate.shape[-1]
+    if gate.is_contiguous() or gate.dim() < 2:
+        return gate.contiguous(), dim
+    stride = want = gate.stride(-2)
+    ok = gate.stride(-1) == 1 and stride >= dim
+    for size, st in zip(reversed(gate.shape[:-1]), reversed(gate.stride()[:-1])):
+        ok = ok and (size == 1 or st == want)
+        want *= size
+    return (gate, stride) if ok else (gate.contiguous(), dim)
 
 
 def _block_norm_args(x, residual, post_weight, gate, scale, pre_weight, eps, activation, post_norm):
     """The checked arguments of m3_block_norm, and the tensors they point into."""
-    if not x.is_cuda:
+    dev = x.get_device()
+    if dev < 0:
         raise ArgumentError(f"x must be a ROCm device tensor (got {x.device}); there is no CPU path")
-    if x.dtype not in _TYPES:
+    code = _TYPES.get(x.dtype)
+    if code is None:
         raise UnsupportedError(f"unsupported: storage dtype {x.dtype}; use float32, bfloat16 or float16")
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ArgumentError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    if x.dim() == 0:
+    shape = x.shape
+    if len(shape) == 0:
         raise ShapeError("shape error: a block norm takes rows, got a scalar")
-    dim = x.shape[-1]
-    if tuple(residual.shape) != tuple(x.shape):
+    dim = shape[-1]
+    if residual.shape != shape:
         raise ShapeError(f"shape error: residual has shape {list(residual.shape)}, expected "
-                         f"{list(x.shape)}")
-    if residual.dtype not in (x.dtype, torch.float32):
+                         f"{list(shape)}")
+    if residual.dtype != x.dtype and residual.dtype != torch.float32:
         raise UnsupportedError("unsupported: the residual stream is in x's type or in float32, got "
                                f"{residual.dtype}")
-    for t, what in ((residual, "residual"), (gate, "gate"), (post_weight, "post_weight"),
-                    (scale, "scale"), (pre_weight, "pre_weight")):
-        if t is not None and t.device != x.device:
-            raise ArgumentError(f"{what} is on {t.device}, x on {x.device}")
+    if residual.get_device() != dev:
+        raise ArgumentError(f"residual is on {residual.device}, x on {x.device}")
     x, residual = x.contiguous(), residual.contiguous()
-    gate_stride = dim
+    gate_stride, gate_ptr = dim, None
     if gate is not None:
-        if gate.dtype != x.dtype:
-            raise ShapeError(f"shape error: gate is {gate.dtype} but x is {x.dtype}")
-        gate, gate_stride = _gate_rows(gate, x.shape)
-    weights = []
+        if gate.dtype != x.dtype or gate.shape != shape:
+            raise ShapeError(f"shape error: gate is {gate.dtype} {list(gate.shape)}, expected {x.dtype} "
+                             f"{list(shape)}")
+        if gate.get_device() != dev:
+            raise ArgumentError(f"gate is on {gate.device}, x on {x.device}")
+        gate, gate_stride = _gate_rows(gate)
+        gate_ptr = gate.data_ptr()
+    weights, ptrs = [], []
     for t, what in ((post_weight, "post_weight"), (scale, "scale"), (pre_weight, "pre_weight")):
         if t is not None:
-            if tuple(t.shape) != (dim,):
+            if t.dim() != 1 or t.shape[0] != dim:
                 raise ShapeError(f"shape error: {what} has shape {list(t.shape)}, expected [{dim}]")
+            if t.get_device() != dev:
+                raise ArgumentError(f"{what} is on {t.device}, x on {x.device}")
             t = t.float().contiguous()
         weights.append(t)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    rows = x.numel() // dim if dim else 0
-    args = _lib.BlockNormC(rows, dim, _TYPES[x.dtype], _TYPES[residual.dtype], int(bool(post_norm)),
-                           _ACTIVATIONS[activation], float(eps), x.data_ptr(), residual.data_ptr(),
-                           ptr(gate), gate_stride, *(ptr(t) for t in weights))
+        ptrs.append(None if t is None else t.data_ptr())
+    args = _lib.BlockNormC(x.numel() // dim if dim else 0, dim, code, _TYPES[residual.dtype],
+                           1 if post_norm else 0, act, eps, x.data_ptr(), residual.data_ptr(), gate_ptr,
+                           gate_stride, *ptrs)
     return args, (x, residual, gate, *weights)
 
 

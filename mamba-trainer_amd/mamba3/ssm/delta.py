@@ -79,68 +79,73 @@ class DeltaGrads:
     h0: Optional[torch.Tensor]
 
 
-def _rows(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None):
-    """(tensor, elements between tokens) of a [B, T, heads, width] tensor: in
-    place where its tokens' rows are contiguous and evenly spaced, else a
-    contiguous copy."""
-    if not t.is_cuda:
-        raise ArgumentError(f"{what} must be a ROCm device tensor (got {t.device}); "
-                            "the delta rule has no CPU path")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ShapeError(f"shape error: {what} is {t.dtype} on {t.device} but v is {like.dtype} on "
-                         f"{like.device}")
-    B, T, H, W = t.shape
+def _rows(t: torch.Tensor, tokens: int, heads: int, width: int):
+    """(tensor, elements between tokens) of a [B, T, heads, width] tensor, or of
+    [B, heads, width] for one token a sequence: in place where its tokens' rows
+    are contiguous and evenly spaced, else a contiguous copy."""
+    row = heads * width
+    if t.is_contiguous():
+        return t, row
     st = t.stride()
-    ok = ((W == 1 or st[3] == 1) and (H == 1 or st[2] == W) and (T == 1 or st[1] >= H * W)
-          and (B == 1 or st[0] == T * st[1]))
-    if T == 1 and B > 1:      # a token's spacing is the sequence's
-        ok = ok and st[0] >= H * W
-        step = st[0]
+    batch = t.shape[0]
+    ok = (width == 1 or st[-1] == 1) and (heads == 1 or st[-2] == width)
+    if tokens == 1:           # a token's spacing is the sequence's
+        step = st[0] if batch > 1 else row
     else:
-        step = st[1] if T > 1 else H * W
-    if not ok or t.numel() == 0:
-        t = t.contiguous()
-        step = H * W
+        step = st[1]
+        ok = ok and (batch == 1 or st[0] == tokens * step)
+    if not ok or step < row or t.numel() == 0:
+        return t.contiguous(), row
     return t, step
 
 
-def _args(inputs: DeltaInputs):
-    """The checked m3_delta_inputs, the tensors it points into, and [B,T,H,P,N,G]."""
-    v = inputs.v
-    if v.dim() != 4:
-        raise RankError(4, v.dim(), v.shape)
-    for t in (inputs.q, inputs.k):
-        if t.dim() != 4:
-            raise RankError(4, t.dim(), t.shape)
-    B, T, H, P = v.shape
-    G, N = inputs.k.shape[2], inputs.k.shape[3]
+def _args(inputs: DeltaInputs, step: bool = False):
+    """The checked m3_delta_inputs, the tensors it points into, and (B, T, H, P, N, G).
+    step: the tensors are of one token a sequence, without the T axis."""
+    q, k, v, g, beta = inputs.q, inputs.k, inputs.v, inputs.g, inputs.beta
+    rank = 3 if step else 4
+    for t in (v, q, k):
+        if t.dim() != rank:
+            raise RankError(rank, t.dim(), t.shape)
+    shape = v.shape
+    B, H, P = shape[0], shape[-2], shape[-1]
+    T = 1 if step else shape[1]
+    G, N = k.shape[-2], k.shape[-1]
     code = _dtype_code(v)
-    _expect_shape(inputs.q, (B, T, G, N), "q")
-    _expect_shape(inputs.k, (B, T, G, N), "k")
-    v, vs = _rows(v, "v")
-    q, qs = _rows(inputs.q, "q", v)
-    k, ks = _rows(inputs.k, "k", v)
-    g, beta = _f32(inputs.g, "g"), _f32(inputs.beta, "beta")
-    _expect_shape(g, (B, T, H), "g")
-    _expect_shape(beta, (B, T, H), "beta")
-    lengths = inputs.lengths
+    lead = (B,) if step else (B, T)
+    dev = v.get_device()
+    for t, what in ((q, "q"), (k, "k")):
+        _expect_shape(t, lead + (G, N), what)
+        if t.dtype != v.dtype or t.get_device() != dev:
+            raise ShapeError(f"shape error: {what} is {t.dtype} on {t.device} but v is {v.dtype} on "
+                             f"{v.device}")
+    if dev < 0:
+        raise ArgumentError(f"v must be a ROCm device tensor (got {v.device}); "
+                            "the delta rule has no CPU path")
+    v, vs = _rows(v, T, H, P)
+    q, qs = _rows(q, T, G, N)
+    k, ks = _rows(k, T, G, N)
+    g, beta = _f32(g, "g"), _f32(beta, "beta")
+    _expect_shape(g, lead + (H,), "g")
+    _expect_shape(beta, lead + (H,), "beta")
+    lengths, h0 = inputs.lengths, _f32(inputs.state, "state")
     if lengths is not None:
         _expect_shape(lengths, (B,), "lengths")
         if not lengths.is_cuda:
             raise ArgumentError("lengths must be a ROCm device tensor")
         lengths = lengths.to(torch.int32).contiguous()
-    h0 = _f32(inputs.state, "state")
     if h0 is not None:
         _expect_shape(h0, (B, H, P, N), "state")
     for t, what in ((g, "g"), (beta, "beta"), (lengths, "lengths"), (h0, "state")):
-        if t is not None and t.device != v.device:
+        if t is not None and t.get_device() != dev:
             raise ArgumentError(f"{what} is on {t.device}, v on {v.device}")
-    scale = N ** -0.5 if inputs.scale is None and N > 0 else (inputs.scale or 0.0)
+    scale = inputs.scale
+    if scale is None:
+        scale = N ** -0.5 if N > 0 else 0.0
     cin = _lib.DeltaInputsC(B, T, H, G, P, N, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks,
                             vs, g.data_ptr(), beta.data_ptr(),
                             None if lengths is None else lengths.data_ptr(),
-                            None if h0 is None else h0.data_ptr(), float(scale),
-                            int(bool(inputs.qk_norm)), None, 0)
+                            None if h0 is None else h0.data_ptr(), scale, 1 if inputs.qk_norm else 0)
     return cin, (q, k, v, g, beta, lengths, h0), (B, T, H, P, N, G)
 
 
@@ -233,18 +238,14 @@ def delta_step_(q, k, v, g, beta, state: torch.Tensor, *, scale: Optional[float]
     """One token a sequence: q, k [B, G, N], v [B, H, P], g, beta [B, H]; `state`
     [B, H, P, N] (f32) is updated IN PLACE; returns y [B, H, P].  A sequence
     whose lengths entry is 0 keeps its state (an empty slot of a batch)."""
-    if v.dim() != 3:
-        raise RankError(3, v.dim(), v.shape)
-    for t in (q, k):
-        if t.dim() != 3:
-            raise RankError(3, t.dim(), t.shape)
-    inputs = DeltaInputs(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), g.unsqueeze(1), beta.unsqueeze(1))
+    inputs = DeltaInputs(q, k, v, g, beta)
     inputs.scale, inputs.qk_norm, inputs.lengths = scale, qk_norm, lengths
-    cin, keep, (B, _, H, P, N, _) = _args(inputs)
+    cin, keep, (B, _, H, P, N, _) = _args(inputs, step=True)
     v = keep[2]
-    if (state.dtype != torch.float32 or not state.is_contiguous() or state.device != v.device):
+    if (state.dtype != torch.float32 or not state.is_contiguous()
+            or state.get_device() != v.get_device()):
         raise ArgumentError(f"state must be a contiguous float32 tensor on {v.device}")
     _expect_shape(state, (B, H, P, N), "state")
-    y = torch.empty((B, H, P), dtype=v.dtype, device=v.device)
+    y = v.new_empty((B, H, P))
     _lib.check(_lib.lib().m3_delta_step(C.byref(cin), state.data_ptr(), y.data_ptr(), _stream(v)))
     return y
