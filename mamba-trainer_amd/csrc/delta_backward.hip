@@ -27,62 +27,72 @@ namespace {
 
 using namespace delta;
 
-// One workgroup a (sequence, head, 64 columns of P), a wave 16 of them, the
-// chunks from the last to the first.
+// One workgroup a (sequence, head, 32 columns of P), the chunks from the last to
+// the first, in pairs of waves as delta_chunks: a wave has half of N of its
+// sixteen columns of the state's gradient.
 template <typename T, int N, bool VEC>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chunks, float *kept) {
-    constexpr int KP = Parts<T>::in, KS = N / 32, NT = N / 16;
+    constexpr int KP = Parts<T>::in, KS = N / 64, NT = N / 32;   // of this wave
     using St = Stage<T, N, VEC, true, 1 + 2 * kTriT, kTriT>;
     constexpr bool DMA = St::DMA;
+    constexpr int BUFS = DMA ? 2 : 1;
     constexpr size_t rec_bytes = BackRecord::units * 1024;
-    __shared__ __attribute__((aligned(1024))) typename St::Buf staged[DMA ? 2 : 1];
+    __shared__ __attribute__((aligned(1024))) typename St::Rows1 sk[BUFS], sq[BUFS];
+    __shared__ __attribute__((aligned(1024))) typename St::Rec sr[BUFS];
+    __shared__ __attribute__((aligned(1024))) typename St::V sv;
+    __shared__ f32x4 meet[4][4][64];
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave >> 1, half = wave & 1;
     const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
-    const int p0 = blockIdx.y * 64, p = p0 + 16 * w + c;      // this lane's column
+    const int p0 = blockIdx.y * kCols, p = p0 + 16 * w + c;      // this lane's column
     const size_t pv = a.heads * P, row0 = (b * L * a.heads + h) * P;
     T *dvp = static_cast<T *>(gr.dv) + row0;
     const uint32_t dv_at = row_off<T>(pv, P, 4 * g, p);
     const Kept kd(a);
+    const int nt0 = half * NT, kk0 = half * KS;
     f32x4 S[NT];   // the gradient of the state after the chunk
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt, g, r);
+            const int n = state_n(nt0 + nt, g, r);
             S[nt][r] = gr.dstate && p < P && n < n_of ? gr.dstate[(bh * P + p) * n_of + n] : 0.f;
         }
     const int live = (len + kC - 1) / kC;
     St in(a, b, h, len, static_cast<const T *>(gr.dy) + row0, pv, p0, records + bh * chunks * rec_bytes, rec_bytes);
     if (live > 0) {
         if constexpr (DMA) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) in.dma(staged[(live - 1) & 1], live - 1, i);
+            in.dma_k(sk[(live - 1) & 1], live - 1);
+            in.dma_q(sq[(live - 1) & 1], live - 1);
+            in.dma_v(sv, live - 1);
+            in.dma_rec(sr[(live - 1) & 1], live - 1);
         } else {
             in.fetch(live - 1);
         }
     }
     for (int ck = live - 1; ck >= 0; --ck) {
-        typename St::Buf &st = staged[DMA ? ck & 1 : 0], &next = staged[DMA ? (ck + 1) & 1 : 0];
+        const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
+        const typename St::Rows1 &k = sk[now], &q1 = sq[now];
+        const unsigned char *rec = sr[now].at;
         f32x4 dy[4];
         if constexpr (DMA) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         } else {
             __syncthreads();
-            in.put(st);
-            in.values(st, dy);
+            in.put(sk[0], sq[0], sr[0]);
+            in.values(sv, dy);
             __syncthreads();
             if (ck > 0) in.fetch(ck - 1);
         }
         float *keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<f32x4 *>(keep + kd.s1() + p * N + state_n(nt, g, 0)) = S[nt];
-        const float *fac = reinterpret_cast<const float *>(st.rec);
+            *reinterpret_cast<f32x4 *>(keep + kd.s1() + p * N + state_n(nt0 + nt, g, 0)) = S[nt];
+        const float *fac = reinterpret_cast<const float *>(rec);
         f32x4 ks[4], x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = ks[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -91,7 +101,7 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int q = 0; q < KP; ++q) kf[kk & 1][i][q] = tile_rows<N>(st.k[q], i, kk, lane);
+                for (int q = 0; q < KP; ++q) kf[kk & 1][i][q] = tile_rows<N>(k.part[q], i, kk0 + kk, lane);
         };
         rows(0);
         split_tiles<kNP>(S[0], S[1], sp[0]);
@@ -100,21 +110,19 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             if (kk + 1 < KS) {
                 rows(kk + 1);
             } else {
-                tri_load<kNP>(st.rec + (1 + kTriT) * 1024, lane, p4, p2, true);
-                if constexpr (DMA) in.values(st, dy);
+                tri_load<kNP>(rec + (1 + kTriT) * 1024, lane, p4, p2, true);
+                if constexpr (DMA) in.values(sv, dy);
             }
-            if constexpr (DMA) {
-                if (ck > 0)
-#pragma unroll
-                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) in.dma(next, ck - 1, i);
-            }
+            if constexpr (DMA)
+                if (ck > 0 && kk == 0) in.dma_k(sk[nxt], ck - 1);
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
             interleave<4 * 3, 5>();
             __builtin_amdgcn_sched_barrier(0);
         }
-        tri_load<kNP>(st.rec + 1024, lane, t4, t2, true);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) meet[wave][i][lane] = ks[i];
         {
             bf16x8 d[2][KP];
             split_tiles<KP>(dy[0], dy[1], d[0]);
@@ -122,8 +130,19 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             mma_rows<2, kNP, KP>(p2, d[0], x);
             mma_rows<4, kNP, KP>(p4, d[1], x);
         }
+        tri_load<kNP>(rec + 1024, lane, t4, t2, true);
+        scan::lds_barrier();
+        if constexpr (DMA)
+            if (ck > 0) {
+                in.dma_q(sq[nxt], ck - 1);
+                in.dma_v(sv, ck - 1);
+                in.dma_rec(sr[nxt], ck - 1);
+            }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += *reinterpret_cast<const f32x4 *>(fac + kFacU + 16 * i + 4 * g) * ks[i];
+        for (int i = 0; i < 4; ++i) {
+            ks[i] += meet[wave ^ 1][i][lane];
+            x[i] += *reinterpret_cast<const f32x4 *>(fac + kFacU + 16 * i + 4 * g) * ks[i];
+        }
         bf16x8 xs[2][kNP], ys[2][kNP];
         split_tiles<kNP>(x[0], x[1], xs[0]);
         split_tiles<kNP>(x[2], x[3], xs[1]);
@@ -131,14 +150,30 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         for (int i = 0; i < 4; ++i) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         mma_rows<2, kNP, kNP>(t2, xs[0], x);
         mma_rows<4, kNP, kNP>(t4, xs[1], x);
-        // x is dR
+        bf16x8 kt[2][NT][KP], qt[2][NT][KP];
+        const auto cols = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int q = 0; q < KP; ++q) {
+                    kt[j][i][q] = tile_cols<N>(k.part[q], nt0 + i, j, lane);
+                    qt[j][i][q] = tile_cols<N>(q1.part[q], nt0 + i, j, lane);
+                }
+        };
+        cols(0);
+        // x is dR: rows 32 half .. are this wave's to write
         const Rows<T, VEC> dvr(dvp + static_cast<size_t>(ck) * kC * pv, pv, len - ck * kC, P);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                keep[kd.dr() + (16 * i + 4 * g + r) * kd.p64 + p] = x[i][r];
-                store_one(dvr, dv_at, 4 * g, p, 16 * i + r, x[i][r]);
+                float v;
+                if (half)
+                    v = x[2 + i][r];
+                else
+                    v = x[i][r];
+                keep[kd.dr() + (32 * half + 16 * i + 4 * g + r) * kd.p64 + p] = v;
+                store_one(dvr, dv_at, 4 * g, p, 32 * half + 16 * i + r, v);
             }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -149,37 +184,27 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         split_tiles<kNP>(x[2], x[3], xs[1]);
         split_tiles<kNP>(dy[0], dy[1], ys[0]);
         split_tiles<kNP>(dy[2], dy[3], ys[1]);
-        bf16x8 kt[2][4][KP], qt[2][4][KP];
-        const auto cols = [&](int j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < KP; ++q) {
-                    kt[j & 1][i][q] = tile_cols<N>(st.k[q], 4 * (j >> 1) + i, j & 1, lane);
-                    qt[j & 1][i][q] = tile_cols<N>(st.q[q], 4 * (j >> 1) + i, j & 1, lane);
-                }
-        };
-        cols(0);
         const float end = fac[kFacEnd];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+        cols(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            if (j + 1 < NT / 2) cols(j + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            mma_rows<4, KP, kNP>(kt[j & 1], xs[j & 1], S + 4 * (j >> 1));
-            mma_rows<4, KP, kNP>(qt[j & 1], ys[j & 1], S + 4 * (j >> 1));
-            __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 2; ++j) {
+            mma_rows<NT, KP, kNP>(kt[j], xs[j], S);
+            mma_rows<NT, KP, kNP>(qt[j], ys[j], S);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (p >= P) return;
-    for (int t = len + g; t < L; t += 4) stf(dvp + t * pv + p, 0.f);
+    if (half == 0)
+        for (int t = len + g; t < L; t += 4) stf(dvp + t * pv + p, 0.f);
     if (gr.dstate0 == nullptr) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt, g, r);
+            const int n = state_n(nt0 + nt, g, r);
             if (n < n_of) gr.dstate0[(bh * P + p) * n_of + n] = S[nt][r];
         }
 }
@@ -542,7 +567,7 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                 };
                 xr[q] = __builtin_shufflevector(four(0, piece), four(0, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
                 yr[q] = __builtin_shufflevector(four(1, piece), four(1, piece + 2), 0, 1, 2, 3, 4, 5, 6, 7);
-                const auto acc = [&](int which, int i) { return tile_acc(place(which, q), i, w, lane); };
+                const auto acc = [&](int which, int i) { return tile_acc<64>(place(which, q), i, w, lane); };
                 xt[q] = __builtin_shufflevector(acc(0, 2 * kk), acc(0, 2 * kk + 1), 0, 1, 2, 3, 4, 5, 6, 7);
                 yt[q] = __builtin_shufflevector(acc(1, 2 * kk), acc(1, 2 * kk + 1), 0, 1, 2, 3, 4, 5, 6, 7);
             }
@@ -650,7 +675,7 @@ hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void
         return by_state(a.d_state, [&](auto n) {
             constexpr int N = decltype(n)::value;
             const int chunks = static_cast<int>(chunks_of(a));
-            const dim3 rev(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>((a.head_dim + 63) / 64));
+            const dim3 rev(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>(kept_cols(a)));
             const dim3 own(static_cast<unsigned>(a.batch * a.groups * chunks));
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;

@@ -188,35 +188,46 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
     if constexpr (BACK) emit(BackRecord::tt, full, std::true_type{});
 }
 
-// One workgroup a (sequence, head, 64 columns of P), a wave 16 of them, the
-// chunks in turn.  With KEEP, the backward's way in: no y, but the state before
-// each chunk and its E are kept.
+// One workgroup a (sequence, head, 32 columns of P), the chunks in turn.  A pair
+// of waves has sixteen columns, each half of the state's N: their halves of K S0^T
+// (and of Q S0^T) meet in LDS, then both form E, and each its half of S and of
+// Y's rows.  DMA: what is read first in a chunk (K, v, the record) goes to a
+// second buffer while the one before is multiplied, Q to the buffer it has left.
+// With KEEP, the backward's way in: no y, but the state before each chunk and its
+// E are kept.
 template <typename T, int N, bool VEC, bool KEEP>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept) {
-    constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 32, NT = N / 16;
+    constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 64, NT = N / 32;   // of this wave
     using R = Record<T>;
     constexpr size_t rec_bytes = (KEEP ? BackRecord::units : R::units) * 1024;
     using St = Stage<T, N, VEC, !KEEP, KEEP ? R::p : R::units, 0>;
     constexpr bool DMA = St::DMA;
-    __shared__ __attribute__((aligned(1024))) typename St::Buf staged[DMA ? 2 : 1];
-    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && !KEEP ? 4 : 1][DMA && !KEEP ? kC : 1][16];
+    constexpr int BUFS = DMA ? 2 : 1;
+    __shared__ __attribute__((aligned(1024))) typename St::Rows1 sk[BUFS];
+    __shared__ __attribute__((aligned(1024))) typename St::Rec sr[BUFS];
+    __shared__ __attribute__((aligned(1024))) typename St::V sv[BUFS];
+    __shared__ __attribute__((aligned(1024))) unsigned char sq_[KEEP ? 16 : sizeof(typename St::Rows1)];
+    __shared__ f32x4 meet[4][KEEP ? 4 : 6][64];
+    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && !KEEP ? 4 : 1][DMA && !KEEP ? 32 : 1][16];
+    typename St::Rows1 &sq = reinterpret_cast<typename St::Rows1 &>(sq_);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave >> 1, half = wave & 1;
     const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
-    const int p0 = blockIdx.y * 64, p = p0 + 16 * w + c;      // this lane's column
+    const int p0 = blockIdx.y * kCols, p = p0 + 16 * w + c;      // this lane's column
     T *yp = static_cast<T *>(a.y) + (b * L * a.heads + h) * P;
     const size_t ystep = a.heads * P;
     const uint32_t y_at = row_off<T>(ystep, P, 4 * g, p);
     const Kept kd(a);
+    const int nt0 = half * NT, kk0 = half * KS;
     f32x4 S[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt, g, r);
+            const int n = state_n(nt0 + nt, g, r);
             S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
         }
     const int live = (len + kC - 1) / kC;
@@ -224,22 +235,26 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
           records + bh * chunks * rec_bytes, rec_bytes);
     if (live > 0) {
         if constexpr (DMA) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) in.dma(staged[0], 0, i);
+            in.dma_k(sk[0], 0);
+            if constexpr (!KEEP) in.dma_q(sq, 0);
+            in.dma_v(sv[0], 0);
+            in.dma_rec(sr[0], 0);
         } else {
             in.fetch(0);
         }
     }
     for (int ck = 0; ck < live; ++ck) {
-        typename St::Buf &st = staged[DMA ? ck & 1 : 0], &next = staged[DMA ? (ck + 1) & 1 : 0];
+        const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
+        const typename St::Rows1 &k = sk[now];
+        const unsigned char *rec = sr[now].at;
         f32x4 e[4];
         if constexpr (DMA) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         } else {
             __syncthreads();
-            in.put(st);
-            in.values(st, e);
+            in.put(sk[0], sq, sr[0]);
+            in.values(sv[0], e);
             __syncthreads();
             if (ck + 1 < live) in.fetch(ck + 1);
         }
@@ -248,11 +263,11 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                *reinterpret_cast<f32x4 *>(keep + kd.s0() + p * N + state_n(nt, g, 0)) = S[nt];
+                *reinterpret_cast<f32x4 *>(keep + kd.s0() + p * N + state_n(nt0 + nt, g, 0)) = S[nt];
         }
-        const float *fac = reinterpret_cast<const float *>(st.rec);
-        // R and the state's part of Y: while a k-step is multiplied, the next one's
-        // operands are read and its columns of S are split
+        const float *fac = reinterpret_cast<const float *>(rec);
+        // this half of K S0^T and Q S0^T: while a k-step is multiplied, the next
+        // one's operands are read and its columns of S are split
         f32x4 y[4], ks[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = ks[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -262,8 +277,8 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int q = 0; q < KP; ++q) {
-                    kf[kk & 1][i][q] = tile_rows<N>(st.k[q], i, kk, lane);
-                    if constexpr (!KEEP) qf[kk & 1][i][q] = tile_rows<N>(st.q[q], i, kk, lane);
+                    kf[kk & 1][i][q] = tile_rows<N>(k.part[q], i, kk0 + kk, lane);
+                    if constexpr (!KEEP) qf[kk & 1][i][q] = tile_rows<N>(sq.part[q], i, kk0 + kk, lane);
                 }
         };
         bf16x8 t4[4][kNP], t2[2][kNP];
@@ -274,14 +289,13 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             if (kk + 1 < KS) {
                 rows(kk + 1);
             } else {
-                tri_load<kNP>(st.rec + R::t * 1024, lane, t4, t2, false);
-                if constexpr (DMA) in.values(st, e);
+                if constexpr (DMA) in.values(sv[now], e);
             }
-            if constexpr (DMA) {
-                if (ck + 1 < live)
-#pragma unroll
-                    for (int i = kk * 4 / KS; i < (kk + 1) * 4 / KS; ++i) in.dma(next, ck + 1, i);
-            }
+            if constexpr (DMA)
+                if (ck + 1 < live && kk == 0) {
+                    in.dma_k(sk[nxt], ck + 1);
+                    in.dma_v(sv[nxt], ck + 1);
+                }
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
@@ -289,11 +303,29 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             interleave<4 * (3 + 2), 3>();
             __builtin_amdgcn_sched_barrier(0);
         }
+        // the other half
+#pragma unroll
+        for (int i = 0; i < 4; ++i) meet[wave][i][lane] = ks[i];
+        if constexpr (!KEEP)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (half)
+                    meet[wave][4 + i][lane] = y[i];
+                else
+                    meet[wave][4 + i][lane] = y[2 + i];
+            }
+        tri_load<kNP>(rec + R::t * 1024, lane, t4, t2, false);
+        scan::lds_barrier();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            ks[i] += meet[wave ^ 1][i][lane];
             e[i] -= *reinterpret_cast<const f32x4 *>(fac + kFacK + 16 * i + 4 * g) * ks[i];
-            if constexpr (!KEEP) y[i] *= *reinterpret_cast<const f32x4 *>(fac + kFacQ + 16 * i + 4 * g);
         }
+        if constexpr (DMA)
+            if (ck + 1 < live) {
+                if constexpr (!KEEP) in.dma_q(sq, ck + 1);
+                in.dma_rec(sr[nxt], ck + 1);
+            }
         // E = T R
         bf16x8 x[2][kNP];
         split_tiles<kNP>(e[0], e[1], x[0]);
@@ -302,23 +334,38 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         for (int i = 0; i < 4; ++i) e[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         mma_rows<4, kNP, kNP>(t4, x[0], e);
         mma_rows<2, kNP, kNP>(t2, x[1], e + 2);
-        // S, and Y's part within the chunk
-        bf16x8 p4[4][YP], p2[2][YP], xe[2][YP];
-        bf16x8 kt[2][4][KP];    // four tiles of N at one k-step
+        // S, and Y's part within the chunk: rows 32 half ..
+        bf16x8 pb[2][2][YP], xe[2][YP];
+        f32x4 yr[2];
+        bf16x8 kt[2][NT][KP];
         const auto cols = [&](int j) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int q = 0; q < KP; ++q)
-                    kt[j & 1][i][q] = tile_cols<N>(st.k[q], 4 * (j >> 1) + i, j & 1, lane);
+                for (int q = 0; q < KP; ++q) kt[j][i][q] = tile_cols<N>(k.part[q], nt0 + i, j, lane);
         };
         cols(0);
         if constexpr (KEEP) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) keep[kd.e() + (16 * i + 4 * g + r) * kd.p64 + p] = e[i][r];
+                for (int r = 0; r < 4; ++r) {
+                    float *to = keep + kd.e() + (32 * half + 16 * i + 4 * g + r) * kd.p64 + p;
+                    if (half)
+                        *to = e[2 + i][r];
+                    else
+                        *to = e[i][r];
+                }
         } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (half)
+                    yr[i] = y[2 + i];
+                else
+                    yr[i] = y[i];
+                yr[i] = (yr[i] + meet[wave ^ 1][4 + i][lane]) *
+                        *reinterpret_cast<const f32x4 *>(fac + kFacQ + 32 * half + 16 * i + 4 * g);
+            }
             split_tiles<YP>(e[0], e[1], xe[0]);
             split_tiles<YP>(e[2], e[3], xe[1]);
         }
@@ -329,48 +376,49 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         const float end = fac[kFacEnd];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+        cols(1);
+        if constexpr (!KEEP)
 #pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            if (j + 1 < NT / 2)
-                cols(j + 1);
-            else if constexpr (!KEEP)
-                tri_load<YP>(st.rec + R::p * 1024, lane, p4, p2, false);
-            __builtin_amdgcn_sched_barrier(0);
-            mma_rows<4, KP, kNP>(kt[j & 1], x[j & 1], S + 4 * (j >> 1));
-            __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int q = 0; q < YP; ++q)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    pb[0][i][q] = tri_block<YP>(rec + R::p * 1024, half ? 2 + 2 * i : i, q, lane);
+                    pb[1][i][q] = tri_block<YP>(rec + R::p * 1024, 3 + 2 * i, q, lane);   // rows 32 .. only
+                }
+        __builtin_amdgcn_sched_barrier(0);
+        mma_rows<NT, KP, kNP>(kt[0], x[0], S);
+        mma_rows<NT, KP, kNP>(kt[1], x[1], S);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (KEEP) continue;
-        mma_rows<4, YP, YP>(p4, xe[0], y);
-        mma_rows<2, YP, YP>(p2, xe[1], y + 2);
+        mma_rows<2, YP, YP>(pb[0], xe[0], yr);
+        if (half) mma_rows<2, YP, YP>(pb[1], xe[1], yr);
         // padding rows past the buffer's end are dropped
-        const Rows<T, VEC> yr(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
+        const Rows<T, VEC> yrow(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
         if constexpr (DMA && !KEEP) {
-            // the wave's 16 columns through LDS to 16-byte stores
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    sy[w][16 * i + 4 * g + r][c] = from_f32<bf16_t>(y[i][r]).bits;
-            const uint32_t at = row_off<T>(ystep, P, lane >> 1, p0 + 16 * w + 8 * (lane & 1));
+            // the wave's 32 x 16 through LDS to 16-byte stores
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                bst16(*reinterpret_cast<const u32x4 *>(&sy[w][32 * i + (lane >> 1)][8 * (lane & 1)]), yr.r,
-                      at + 32 * i * yr.step);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    sy[wave][16 * i + 4 * g + r][c] = from_f32<bf16_t>(yr[i][r]).bits;
+            bst16(*reinterpret_cast<const u32x4 *>(&sy[wave][lane >> 1][8 * (lane & 1)]), yrow.r,
+                  row_off<T>(ystep, P, 32 * half + (lane >> 1), p0 + 16 * w + 8 * (lane & 1)));
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) store_one(yr, y_at, 4 * g, p, 16 * i + r, y[i][r]);
+                for (int r = 0; r < 4; ++r) store_one(yrow, y_at, 4 * g, p, 32 * half + 16 * i + r, yr[i][r]);
         }
     }
     if (KEEP || p >= P) return;
-    for (int t = len + g; t < L; t += 4) stf(yp + t * ystep + p, 0.f);
+    if (half == 0)
+        for (int t = len + g; t < L; t += 4) stf(yp + t * ystep + p, 0.f);
     if (a.state_out == nullptr) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt, g, r);
+            const int n = state_n(nt0 + nt, g, r);
             if (n < n_of) a.state_out[(bh * P + p) * n_of + n] = S[nt][r];
         }
 }
@@ -383,7 +431,7 @@ hipError_t launch(const DeltaLaunch &a, unsigned char *records, float *kept, hip
             constexpr int N = decltype(n)::value;
             const int chunks = static_cast<int>(chunks_of(a));
             const dim3 prep(static_cast<unsigned>(a.batch * a.heads * chunks));
-            const dim3 main(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>((a.head_dim + 63) / 64));
+            const dim3 main(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>(KEEP ? kept_cols(a) : (a.head_dim + kCols - 1) / kCols));
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
                 hipLaunchKernelGGL((delta_prep<T, N, VEC, KEEP>), prep, dim3(256), 0, s, a, records, chunks);

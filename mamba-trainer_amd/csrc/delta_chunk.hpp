@@ -241,7 +241,7 @@ __device__ __forceinline__ void to_parts(const Eight<T> &r, bf16x8 *out) {
 // (a transposed operand).
 template <int N>
 __device__ __forceinline__ constexpr int swizzle(int t) {
-    return N == 128 ? (t & 3) << 2 | ((t >> 2) & 3) : ((t >> 1) & 1) << 2 | ((t >> 2) & 3);
+    return N == 128 ? (t & 3) << 2 | ((t >> 2) & 3) : N == 64 ? ((t >> 1) & 1) << 2 | ((t >> 2) & 3) : 0;
 }
 template <int N> struct Tile {
     static constexpr int bytes = kC * N * 2;
@@ -265,10 +265,11 @@ __device__ __forceinline__ bf16x8 tile_cols(const unsigned char *t, int nt, int 
     const bf16x4 hi = scan::lds_read_tr16(reinterpret_cast<const __bf16 *>(p + 16 * (2 * N)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// Sixteen columns from 16 w on of a 64-wide tile as accumulator tile i holds them.
+// Sixteen columns from 16 w on of an M-wide tile as accumulator tile i holds them.
+template <int M>
 __device__ __forceinline__ bf16x4 tile_acc(const unsigned char *t, int i, int w, int lane) {
     const int l = lane & 15, g = lane >> 4, q = l & 3;
-    const unsigned char *p = t + 16 * i * 128 + tile_at<64>(4 * g + (l >> 2), 2 * w + (q >> 1)) + 8 * (q & 1);
+    const unsigned char *p = t + 16 * i * (2 * M) + tile_at<M>(4 * g + (l >> 2), 2 * w + (q >> 1)) + 8 * (q & 1);
     return scan::lds_read_tr16(reinterpret_cast<const __bf16 *>(p));
 }
 // The n of row r of lane group g of S's tile nt.
@@ -311,25 +312,26 @@ struct BackRecord {
     static constexpr int t = 1, tt = t + kTriT, pt = tt + kTriT, units = pt + kTriT;
 };
 
-// The fetch of a chunk's operands to LDS: K, Q if WITHQ, a 64-column tile of v
-// (or dy), and UNITS kilobytes of its record (unit u > 0 from kilobyte u + GAP).
-// bf16 with aligned rows (DMA): straight from memory, in four parts that the
-// caller spreads over its products.  Other inputs become their bf16 parts on
-// the way, through registers; v stays in registers.
+// Columns of P that a workgroup of the chunk kernels takes: two tiles, each a
+// pair of waves' whose halves of N meet in LDS.
+constexpr int kCols = 32;
+
+// The fetch of a chunk's operands to LDS: K, Q, a tile of v (or dy), and UNITS
+// kilobytes of its record (unit u > 0 from kilobyte u + GAP).  bf16 with aligned
+// rows (DMA): straight from memory, piece by piece where the caller says.  Other
+// inputs become their bf16 parts on the way, through registers; v stays there.
 template <typename T, int N, bool VEC, bool WITHQ, int UNITS, int GAP>
 struct Stage {
     static constexpr int KP = Parts<T>::in;
     static constexpr bool DMA = VEC && std::is_same<T, bf16_t>::value;
     static constexpr int pieces = kC * N / 8 / 256, rpieces = UNITS / 4 + 1;
-    struct Buf {
-        unsigned char k[KP][Tile<N>::bytes], q[WITHQ ? KP : 1][WITHQ ? Tile<N>::bytes : 16];
-        unsigned char v[DMA ? Tile<64>::bytes : 16];
-        unsigned char rec[UNITS * 1024];
-    };
+    struct Rows1 { unsigned char part[KP][Tile<N>::bytes]; };
+    struct Rec { unsigned char at[UNITS * 1024]; };
+    struct V { unsigned char at[DMA ? Tile<kCols>::bytes : 16]; };
     const T *kp, *qp, *vp;              // the sequence's rows of this head
     size_t ks, qs, vs, rec_bytes;
     const unsigned char *rec;           // the sequence's records
-    int len, n_of, P, w, lane;
+    int len, n_of, P, wave, w, lane;    // wave: of four; w: its tile of columns
     uint32_t dk, dq, dv;                // DMA places
     int kt, kn, vt, vn;                 // else: this thread's places
     uint32_t k_at, q_at, v_at;
@@ -341,7 +343,8 @@ struct Stage {
                                      int p0, const unsigned char *records, size_t record_bytes) {
         const int tid = threadIdx.x;
         lane = tid & 63;
-        w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        w = wave >> 1;
         len = length;
         n_of = static_cast<int>(a.d_state);
         P = static_cast<int>(a.head_dim);
@@ -359,9 +362,9 @@ struct Stage {
         vt = 4 * (lane >> 4);
         vn = p0 + 16 * w + (lane & 15);
         if constexpr (DMA) {
-            dk = dma_at<T, N>(ks, n_of, 0, w, lane);
-            dq = dma_at<T, N>(qs, n_of, 0, w, lane);
-            dv = dma_at<T, 64>(vs, P, p0, w, lane);
+            dk = dma_at<T, N>(ks, n_of, 0, wave, lane);
+            dq = dma_at<T, N>(qs, n_of, 0, wave, lane);
+            dv = dma_at<T, kCols>(vs, P, p0, wave, lane);
         } else {
             k_at = row_off<T>(ks, n_of, kt, kn);
             q_at = row_off<T>(qs, n_of, kt, kn);
@@ -370,28 +373,23 @@ struct Stage {
     }
     __device__ __forceinline__ rsrc_t record(int ck) const { return make_rsrc(rec + ck * rec_bytes, static_cast<uint32_t>(rec_bytes)); }
     static __device__ __forceinline__ constexpr int unit(int u) { return u == 0 ? 0 : u + GAP; }
+    __device__ __forceinline__ Rows<T, VEC> rows_of(const T *p, size_t stride, int ck, int width) const {
+        return Rows<T, VEC>(p + static_cast<size_t>(ck) * kC * stride, stride, len - ck * kC, width);
+    }
 
-    __device__ __forceinline__ void dma(Buf &to, int ck, int part) const {
-        const size_t t0 = static_cast<size_t>(ck) * kC;
-        const int left = len - ck * kC;
-        if (part == 0) dma_tile<N>(Rows<T, true>(kp + t0 * ks, ks, left, n_of), dk, to.k[0], w);
-        if (part == 1 && WITHQ) dma_tile<N>(Rows<T, true>(qp + t0 * qs, qs, left, n_of), dq, to.q[0], w);
-        if (part == 2) dma_tile<64>(Rows<T, true>(vp + t0 * vs, vs, left, P), dv, to.v, w);
-        if (part >= 2) {
-            const rsrc_t r = record(ck);
-            constexpr int half = (UNITS + 7) / 8;
+    __device__ __forceinline__ void dma_k(Rows1 &to, int ck) const { dma_tile<N>(rows_of(kp, ks, ck, n_of), dk, to.part[0], wave); }
+    __device__ __forceinline__ void dma_q(Rows1 &to, int ck) const { dma_tile<N>(rows_of(qp, qs, ck, n_of), dq, to.part[0], wave); }
+    __device__ __forceinline__ void dma_v(V &to, int ck) const { dma_tile<kCols>(rows_of(vp, vs, ck, P), dv, to.at, wave); }
+    __device__ __forceinline__ void dma_rec(Rec &to, int ck) const {
+        const rsrc_t r = record(ck);
 #pragma unroll
-            for (int i = 0; i < half; ++i) {
-                const int u = w + 4 * (i + (part - 2) * half);
-                if (u < UNITS) scan::lds_dma16(r, scan::lds_addr(to.rec + u * 1024), unit(u) * 1024 + lane * 16);
-            }
+        for (int i = 0; i < rpieces; ++i) {
+            const int u = wave + 4 * i;
+            if (u < UNITS) scan::lds_dma16(r, scan::lds_addr(to.at + u * 1024), unit(u) * 1024 + lane * 16);
         }
     }
     __device__ __forceinline__ void fetch(int ck) {
-        const size_t t0 = static_cast<size_t>(ck) * kC;
-        const int left = len - ck * kC;
-        const Rows<T, VEC> kr(kp + t0 * ks, ks, left, n_of), qr(qp + t0 * qs, qs, left, n_of);
-        const Rows<T, VEC> vr(vp + t0 * vs, vs, left, P);
+        const Rows<T, VEC> kr = rows_of(kp, ks, ck, n_of), qr = rows_of(qp, qs, ck, n_of), vr = rows_of(vp, vs, ck, P);
 #pragma unroll
         for (int i = 0; i < pieces; ++i) {
             k8[i] = load_eight(kr, k_at, kt, kn, i * (2048 / N));
@@ -399,36 +397,36 @@ struct Stage {
         }
         const rsrc_t r = record(ck);
 #pragma unroll
-        for (int i = 0; i < rpieces; ++i) r8[i] = bld16(r, unit(w + 4 * i) * 1024 + lane * 16);
+        for (int i = 0; i < rpieces; ++i) r8[i] = bld16(r, unit(wave + 4 * i) * 1024 + lane * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int r1 = 0; r1 < 4; ++r1) v1[i][r1] = load_one(vr, v_at, vt, vn, 16 * i + r1);
     }
-    __device__ __forceinline__ void put(Buf &to) const {
+    __device__ __forceinline__ void put(Rows1 &k, Rows1 &q, Rec &to) const {
 #pragma unroll
         for (int i = 0; i < pieces; ++i) {
             bf16x8 x[KP];
             const int at = tile_at<N>(kt + i * (2048 / N), kn / 8);
             to_parts(k8[i], x);
 #pragma unroll
-            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(to.k[q] + at) = x[q];
+            for (int p = 0; p < KP; ++p) *reinterpret_cast<bf16x8 *>(k.part[p] + at) = x[p];
             if constexpr (WITHQ) {
                 to_parts(q8[i], x);
 #pragma unroll
-                for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(to.q[q] + at) = x[q];
+                for (int p = 0; p < KP; ++p) *reinterpret_cast<bf16x8 *>(q.part[p] + at) = x[p];
             }
         }
 #pragma unroll
         for (int i = 0; i < rpieces; ++i)
-            if (w + 4 * i < UNITS) *reinterpret_cast<u32x4 *>(to.rec + (w + 4 * i) * 1024 + lane * 16) = r8[i];
+            if (wave + 4 * i < UNITS) *reinterpret_cast<u32x4 *>(to.at + (wave + 4 * i) * 1024 + lane * 16) = r8[i];
     }
     // v as accumulator tiles
-    __device__ __forceinline__ void values(const Buf &from, f32x4 *e) const {
+    __device__ __forceinline__ void values(const V &from, f32x4 *e) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (DMA) {
-                const bf16x4 x = tile_acc(from.v, i, w, lane);
+                const bf16x4 x = tile_acc<kCols>(from.at, i, w, lane);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) e[i][r] = static_cast<float>(x[r]);
             } else {
@@ -482,6 +480,9 @@ struct Kept {
     __host__ __device__ size_t dr() const { return 2 * p64 * n + kC * p64; }
     __host__ __device__ size_t floats() const { return 2 * p64 * (n + kC); }
 };
+
+// The backward's chunk kernels write all of P64.
+inline size_t kept_cols(const DeltaLaunch &a) { return Kept(a).p64 / kCols; }
 
 // delta_prep and the forward states of the backward (delta_chunk.hip).
 hipError_t launch_delta_states(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s, int &launches);

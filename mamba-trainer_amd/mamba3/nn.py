@@ -258,7 +258,8 @@ def _block_norm_args(x, residual, post_weight, gate, scale, pre_weight, eps, act
                 raise ShapeError(f"shape error: {what} has shape {list(t.shape)}, expected [{dim}]")
             if t.get_device() != dev:
                 raise ArgumentError(f"{what} is on {t.device}, x on {x.device}")
-            t = t.float().contiguous()
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                t = t.float().contiguous()
         weights.append(t)
         ptrs.append(None if t is None else t.data_ptr())
     args = _lib.BlockNormC(x.numel() // dim if dim else 0, dim, code, _TYPES[residual.dtype],
@@ -282,7 +283,12 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor, *, post_weight=None, gat
     factor.  A gate whose rows are columns of a wider row is read in place.
     Differentiable."""
     tensors = (x, residual, gate, post_weight, scale, pre_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or residual.requires_grad
+            or (gate is not None and gate.requires_grad)
+            or (post_weight is not None and post_weight.requires_grad)
+            or (scale is not None and scale.requires_grad)
+            or (pre_weight is not None and pre_weight.requires_grad)):
         r, y = _BlockNormFn.apply((eps, activation, post_norm, normed), *tensors)
         return r, y
     return _block_norm_forward(tensors, eps, activation, post_norm, normed)
