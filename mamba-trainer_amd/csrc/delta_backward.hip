@@ -648,26 +648,23 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
     }
 }
 
-size_t align256(size_t v) { return (v + 255) / 256 * 256; }
-
-size_t records_bytes(const DeltaLaunch &a) {
-    return align256(a.batch * a.heads * chunks_of(a) * BackRecord::units * 1024);
-}
-
 }  // namespace
 
 bool delta_backward_supported(const DeltaLaunch &a) { return a.d_state <= 128; }
 
 size_t delta_backward_workspace(const DeltaLaunch &a) {
-    return records_bytes(a) + a.batch * a.heads * chunks_of(a) * Kept(a).floats() * sizeof(float);
+    size_t kept_at = 0;
+    return delta_states_workspace(a, kept_at);
 }
 
 hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void *workspace, hipStream_t s,
                                  int &launches) {
     unsigned char *records = static_cast<unsigned char *>(workspace);
-    float *kept = reinterpret_cast<float *>(records + records_bytes(a));
+    size_t kept_at = 0;
+    delta_states_workspace(a, kept_at);
+    float *kept = reinterpret_cast<float *>(records + kept_at);
     if (a.seq > 0) {
-        const hipError_t e = launch_delta_states(a, records, kept, s, launches);
+        const hipError_t e = launch_delta_states(a, records, s, launches);
         if (e != hipSuccess) return e;
     }
     return by_type(a.dtype, [&](auto t) {

@@ -10,14 +10,18 @@ using namespace delta;
 // One workgroup a (sequence, head, chunk): the chunk's row factors, T and the
 // attention within the chunk.
 template <typename T, int N, bool VEC, bool BACK>
-__global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *records, int chunks) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta_prep(DeltaLaunch a, unsigned char *records, int chunks) {
     constexpr int KP = Parts<T>::in, LP = kC + 4;
     using R = Record<T>;
     constexpr size_t bytes = (BACK ? BackRecord::units : R::units) * 1024;
+    // the rows as loaded, then (in the same place) the triangles
+    constexpr int row_bytes = N * sizeof(T), rows_bytes = kC * row_bytes, tri_bytes = kC * LP * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char area[2 * (rows_bytes > tri_bytes ? rows_bytes : tri_bytes)];
     __shared__ double G[kC];
     __shared__ float beta[kC], rq[kC], rk[kC];
-    __shared__ __attribute__((aligned(16))) float A[kC][LP], X[kC][LP];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+    float(*A)[LP] = reinterpret_cast<float(*)[LP]>(area), (*X)[LP] = A + kC;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t rec = blockIdx.x, bh = rec / chunks, b = bh / a.heads, h = bh % a.heads;
     const int t0 = static_cast<int>(rec % chunks) * kC;
     const int L = static_cast<int>(a.seq), live = valid_len(a.lengths, b, L) - t0;   // of this chunk
@@ -26,6 +30,36 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
     const int n_of = static_cast<int>(a.d_state);
     const Rows<T, VEC> kp(static_cast<const T *>(a.k) + (b * L + t0) * a.ks + kg * n_of, a.ks, live, n_of);
     const Rows<T, VEC> qp(static_cast<const T *>(a.q) + (b * L + t0) * a.qs + kg * n_of, a.qs, live, n_of);
+    // eight values of row t from n on: 16-byte pieces, permuted against bank conflicts
+    const auto at = [&](int which, int t, int n) {
+        const int piece = n * sizeof(T) / 16, perm = sizeof(T) == 4 ? t & 15 : swizzle<N>(t);
+        return area + which * rows_bytes + t * row_bytes + ((piece ^ perm) << 4);
+    };
+    const auto put = [&](int which, int t, int n, const Eight<T> &e) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<u32x4 *>(at(which, t, n)) = e.a;
+            *reinterpret_cast<u32x4 *>(at(which, t, n + 4)) = e.b;
+        } else {
+            *reinterpret_cast<u32x4 *>(at(which, t, n)) = e.q;
+        }
+    };
+    const auto get = [&](int which, int t, int n, bf16x8 *out) {
+        Eight<T> e;
+        if constexpr (sizeof(T) == 4) {
+            e.a = *reinterpret_cast<const u32x4 *>(at(which, t, n));
+            e.b = *reinterpret_cast<const u32x4 *>(at(which, t, n + 4));
+        } else {
+            e.q = *reinterpret_cast<const u32x4 *>(at(which, t, n));
+        }
+        to_parts(e, out);
+    };
+    constexpr int per = N / 8, pieces = kC * per / 256;   // threads of a row
+    Eight<T> k8[pieces], q8[pieces];
+#pragma unroll
+    for (int i = 0; i < pieces; ++i) {
+        k8[i] = load_eight(kp, tid / per + i * (256 / per), tid % per * 8);
+        q8[i] = load_eight(qp, tid / per + i * (256 / per), tid % per * 8);
+    }
     if (w == 0) {
         const size_t th = (b * L + t0 + lane) * a.heads + h;
         double s = 0.0;
@@ -42,62 +76,75 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
         G[lane] = s;
         beta[lane] = bt;
     }
-    // Q and K rows of this wave's 16 tokens as operands, their lengths
-    bf16x8 qa[N / 32][KP], ka[N / 32][KP];
-    const int my = 16 * w + c;
-    float sq = 0.f, sk = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < N / 32; ++kk) {
-        const Eight<T> q8 = load_eight(qp, my, 32 * kk + 8 * g);
-        const Eight<T> k8 = load_eight(kp, my, 32 * kk + 8 * g);
-        float f[8];
-        widen(q8, f);
+    for (int i = 0; i < pieces; ++i) {
+        const int t = tid / per + i * (256 / per), n = tid % per * 8;
+        float f[8], sq = 0.f, sk = 0.f;
+        widen(q8[i], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq += f[i] * f[i];
-        widen(k8, f);
+        for (int e = 0; e < 8; ++e) sq += f[e] * f[e];
+        widen(k8[i], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sk += f[i] * f[i];
-        to_parts(q8, qa[kk]);
-        to_parts(k8, ka[kk]);
-    }
-    sq += __shfl_xor(sq, 16, 64);
-    sk += __shfl_xor(sk, 16, 64);
-    sq += __shfl_xor(sq, 32, 64);
-    sk += __shfl_xor(sk, 32, 64);
-    if (g == 0) {
-        rq[my] = a.scale * (a.qk_norm ? 1.0f / sqrtf(sq + kUnitEps) : 1.0f);
-        rk[my] = a.qk_norm ? 1.0f / sqrtf(sk + kUnitEps) : 1.0f;
-    }
-    // tiles j <= w of K K^T and Q K^T
-    f32x4 kkt[4], qkt[4];
+        for (int e = 0; e < 8; ++e) sk += f[e] * f[e];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        kkt[j] = qkt[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (j > w) continue;
-        const int row = 16 * j + c;
-#pragma unroll
-        for (int kk = 0; kk < N / 32; ++kk) {
-            bf16x8 kb[KP];
-            to_parts(load_eight(kp, row, 32 * kk + 8 * g), kb);
-            kkt[j] = mma_parts<KP, KP>(ka[kk], kb, kkt[j]);
-            qkt[j] = mma_parts<KP, KP>(qa[kk], kb, qkt[j]);
+        for (int off = 1; off < per; off <<= 1) {
+            sq += __shfl_xor(sq, off, 64);
+            sk += __shfl_xor(sk, off, 64);
         }
+        if (n == 0) {
+            rq[t] = a.scale * (a.qk_norm ? 1.0f / sqrtf(sq + kUnitEps) : 1.0f);
+            rk[t] = a.qk_norm ? 1.0f / sqrtf(sk + kUnitEps) : 1.0f;
+        }
+        put(0, t, n, k8[i]);
+        put(1, t, n, q8[i]);
     }
     __syncthreads();
+    // the ten lower tiles of K K^T and Q K^T, two or three a wave: (0,0) (3,0) (3,1);
+    // (1,0) (1,1); (2,0) (2,1) (2,2); (3,2) (3,3)
+    const int count = w & 1 ? 2 : 3;
+    const auto row_of = [&](int s) { return w == 0 && s > 0 ? 3 : w; };
+    const auto col_of = [&](int s) { return w == 0 ? (s > 0 ? s - 1 : 0) : w == 3 ? 2 + s : s; };
+    f32x4 kkt[3], qkt[3];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int s = 0; s < 3; ++s) {
+        kkt[s] = qkt[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s >= count) continue;
+        const int ri = 16 * row_of(s) + c, rj = 16 * col_of(s) + c;
+#pragma unroll
+        for (int kk = 0; kk < N / 32; ++kk) {
+            bf16x8 qa[KP], ka[KP], kb[KP];
+            get(1, ri, 32 * kk + 8 * g, qa);
+            get(0, ri, 32 * kk + 8 * g, ka);
+            get(0, rj, 32 * kk + 8 * g, kb);
+            kkt[s] = mma_parts<KP, KP>(ka, kb, kkt[s]);
+            qkt[s] = mma_parts<KP, KP>(qa, kb, qkt[s]);
+        }
+    }
+    __syncthreads();   // the rows are done with
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+        if (s >= count) continue;
+        const int jj = 16 * col_of(s) + c;
+        const float f = rk[jj] * beta[jj];
+        const double gj = G[jj];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int i = 16 * w + 4 * g + r, jj = 16 * j + c;
+            const int i = 16 * row_of(s) + 4 * g + r;
             float m = 0.f, p = 0.f;
             if (jj <= i) {
-                const float d = expf(static_cast<float>(G[i] - G[jj])) * rk[jj] * beta[jj];
-                p = d * rq[i] * qkt[j][r];
-                if (jj < i) m = d * rk[i] * kkt[j][r];
+                const float d = expf(static_cast<float>(G[i] - gj)) * f;
+                p = d * rq[i] * qkt[s][r];
+                if (jj < i) m = d * rk[i] * kkt[s][r];
             }
             A[i][jj] = m;
             X[i][jj] = p;
         }
+    }
+    // the tiles above the diagonal that an operand block takes in: zero
+    if ((w & 1) == 0)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) X[16 * w + 4 * g + r][16 * (w + 1) + c] = 0.f;
+    const int my = 16 * w + c;
     unsigned char *out = records + rec * bytes;
     if (w == 0) {
         float *f = reinterpret_cast<float *>(out);
@@ -179,10 +226,6 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
 #pragma unroll
                 for (int r = 0; r < 4; ++r) X[16 * (w + d) + 4 * g + r][16 * w + c] = t[d][r];
     }
-    // above the diagonal T is zero where a block row's operands reach past it
-    if ((w & 1) == 0)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) X[16 * w + 4 * g + r][16 * (w + 1) + c] = 0.f;
     __syncthreads();
     emit(R::t, full, std::false_type{});
     if constexpr (BACK) emit(BackRecord::tt, full, std::true_type{});
@@ -193,30 +236,42 @@ __global__ void __launch_bounds__(256) delta_prep(DeltaLaunch a, unsigned char *
 // (and of Q S0^T) meet in LDS, then both form E, and each its half of S and of
 // Y's rows.  DMA: what is read first in a chunk (K, v, the record) goes to a
 // second buffer while the one before is multiplied, Q to the buffer it has left.
-// With KEEP, the backward's way in: no y, but the state before each chunk and its
-// E are kept.
-template <typename T, int N, bool VEC, bool KEEP>
+// KEEP is the backward's way in: no y, but the state before each chunk and its E
+// are kept.
+//
+// Few sequences leave most CUs idle while their chunks pass one by one; then the
+// window is cut into segments that run side by side.  As S [P, N] passes through
+// a segment it becomes S Phi + Psi, with Phi [N, N] of the keys alone, so a CARRY
+// pass finds Psi (the segment on v from a zero state) and Phi (on v = 0 from the
+// rows of the identity, as further columns of P), delta_join the state before
+// each segment, and the window's pass (or KEEP) runs each from there: some
+// (2 P + N) / P times the work, in segments' time.
+enum { kWindow, kKeep, kCarry };
+template <typename T, int N, bool VEC, int MODE, bool BACK>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept) {
+delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept, Segments sg) {
+    constexpr bool KEEP = MODE == kKeep, Y = MODE == kWindow;
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 64, NT = N / 32;   // of this wave
     using R = Record<T>;
-    constexpr size_t rec_bytes = (KEEP ? BackRecord::units : R::units) * 1024;
-    using St = Stage<T, N, VEC, !KEEP, KEEP ? R::p : R::units, 0>;
+    constexpr size_t rec_bytes = (BACK ? BackRecord::units : R::units) * 1024;
+    using St = Stage<T, N, VEC, Y, Y ? R::units : R::p, 0>;
     constexpr bool DMA = St::DMA;
     constexpr int BUFS = DMA ? 2 : 1;
     __shared__ __attribute__((aligned(1024))) typename St::Rows1 sk[BUFS];
     __shared__ __attribute__((aligned(1024))) typename St::Rec sr[BUFS];
     __shared__ __attribute__((aligned(1024))) typename St::V sv[BUFS];
-    __shared__ __attribute__((aligned(1024))) unsigned char sq_[KEEP ? 16 : sizeof(typename St::Rows1)];
-    __shared__ f32x4 meet[4][KEEP ? 4 : 6][64];
-    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && !KEEP ? 4 : 1][DMA && !KEEP ? 32 : 1][16];
+    __shared__ __attribute__((aligned(1024))) unsigned char sq_[!Y ? 16 : sizeof(typename St::Rows1)];
+    __shared__ f32x4 meet[4][Y ? 6 : 4][64];
+    __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && Y ? 4 : 1][DMA && Y ? 32 : 1][16];
     typename St::Rows1 &sq = reinterpret_cast<typename St::Rows1 &>(sq_);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave >> 1, half = wave & 1;
-    const size_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
+    const size_t bh = blockIdx.x / sg.count, b = bh / a.heads, h = bh % a.heads;
+    const int seg = static_cast<int>(blockIdx.x % sg.count);
     const int L = static_cast<int>(a.seq), len = valid_len(a.lengths, b, L);
     const int n_of = static_cast<int>(a.d_state), P = static_cast<int>(a.head_dim);
     const int p0 = blockIdx.y * kCols, p = p0 + 16 * w + c;      // this lane's column
+    const int unit_row = p - static_cast<int>(sg.cols);           // CARRY: of the identity, if not below 0
     T *yp = static_cast<T *>(a.y) + (b * L * a.heads + h) * P;
     const size_t ystep = a.heads * P;
     const uint32_t y_at = row_off<T>(ystep, P, 4 * g, p);
@@ -228,22 +283,28 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int n = state_n(nt0 + nt, g, r);
-            S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
+            if constexpr (MODE == kCarry)
+                S[nt][r] = n == unit_row ? 1.f : 0.f;
+            else if (sg.count > 1)
+                S[nt][r] = sg.starts[((bh * sg.count + seg) * sg.cols + p) * N + n];
+            else
+                S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
         }
-    const int live = (len + kC - 1) / kC;
+    const int all = (len + kC - 1) / kC, first = seg * sg.chunks;
+    const int live = sg.chunks < all - first ? first + sg.chunks : all;   // the segment's end
     St in(a, b, h, len, static_cast<const T *>(a.v) + b * L * a.vs + h * P, a.vs, p0,
           records + bh * chunks * rec_bytes, rec_bytes);
-    if (live > 0) {
+    if (first < live) {
         if constexpr (DMA) {
-            in.dma_k(sk[0], 0);
-            if constexpr (!KEEP) in.dma_q(sq, 0);
-            in.dma_v(sv[0], 0);
-            in.dma_rec(sr[0], 0);
+            in.dma_k(sk[first & 1], first);
+            if constexpr (Y) in.dma_q(sq, first);
+            in.dma_v(sv[first & 1], first);
+            in.dma_rec(sr[first & 1], first);
         } else {
-            in.fetch(0);
+            in.fetch(first);
         }
     }
-    for (int ck = 0; ck < live; ++ck) {
+    for (int ck = first; ck < live; ++ck) {
         const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
         const typename St::Rows1 &k = sk[now];
         const unsigned char *rec = sr[now].at;
@@ -278,7 +339,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
 #pragma unroll
                 for (int q = 0; q < KP; ++q) {
                     kf[kk & 1][i][q] = tile_rows<N>(k.part[q], i, kk0 + kk, lane);
-                    if constexpr (!KEEP) qf[kk & 1][i][q] = tile_rows<N>(sq.part[q], i, kk0 + kk, lane);
+                    if constexpr (Y) qf[kk & 1][i][q] = tile_rows<N>(sq.part[q], i, kk0 + kk, lane);
                 }
         };
         bf16x8 t4[4][kNP], t2[2][kNP];
@@ -299,14 +360,14 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
-            if constexpr (!KEEP) mma_rows<4, KP, YP>(qf[kk & 1], sp[kk & 1], y);
+            if constexpr (Y) mma_rows<4, KP, YP>(qf[kk & 1], sp[kk & 1], y);
             interleave<4 * (3 + 2), 3>();
             __builtin_amdgcn_sched_barrier(0);
         }
         // the other half
 #pragma unroll
         for (int i = 0; i < 4; ++i) meet[wave][i][lane] = ks[i];
-        if constexpr (!KEEP)
+        if constexpr (Y)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (half)
@@ -323,7 +384,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         }
         if constexpr (DMA)
             if (ck + 1 < live) {
-                if constexpr (!KEEP) in.dma_q(sq, ck + 1);
+                if constexpr (Y) in.dma_q(sq, ck + 1);
                 in.dma_rec(sr[nxt], ck + 1);
             }
         // E = T R
@@ -377,7 +438,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
         cols(1);
-        if constexpr (!KEEP)
+        if constexpr (Y)
 #pragma unroll
             for (int q = 0; q < YP; ++q)
 #pragma unroll
@@ -389,12 +450,12 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         mma_rows<NT, KP, kNP>(kt[0], x[0], S);
         mma_rows<NT, KP, kNP>(kt[1], x[1], S);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (KEEP) continue;
+        if constexpr (!Y) continue;
         mma_rows<2, YP, YP>(pb[0], xe[0], yr);
         if (half) mma_rows<2, YP, YP>(pb[1], xe[1], yr);
         // padding rows past the buffer's end are dropped
         const Rows<T, VEC> yrow(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
-        if constexpr (DMA && !KEEP) {
+        if constexpr (DMA && Y) {
             // the wave's 32 x 16 through LDS to 16-byte stores
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -410,10 +471,16 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
                 for (int r = 0; r < 4; ++r) store_one(yrow, y_at, 4 * g, p, 32 * half + 16 * i + r, yr[i][r]);
         }
     }
+    if constexpr (MODE == kCarry) {
+        float *to = sg.carry + ((bh * sg.count + seg) * (sg.cols + N) + p) * N;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<f32x4 *>(to + state_n(nt0 + nt, g, 0)) = S[nt];
+        return;
+    }
     if (KEEP || p >= P) return;
-    if (half == 0)
+    if (half == 0 && seg == 0)
         for (int t = len + g; t < L; t += 4) stf(yp + t * ystep + p, 0.f);
-    if (a.state_out == nullptr) return;
+    if (a.state_out == nullptr || seg + 1 < static_cast<int>(sg.count)) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -423,19 +490,132 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         }
 }
 
-template <bool KEEP>
-hipError_t launch(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s, int &launches) {
+// The state before each segment: one workgroup a (sequence, head, 16 rows of S),
+// a wave 16 columns, S_s Phi_s + Psi_s segment by segment in f32 (MFMA 16x16x4);
+// the next segment's Phi and Psi are on their way meanwhile.
+template <int N>
+__global__ void __launch_bounds__(4 * N) delta_join(DeltaLaunch a, Segments sg) {
+    constexpr int KS = N / 4;
+    __shared__ float s[2][16][N + 4];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+    const size_t bh = blockIdx.x;
+    const int p0 = blockIdx.y * 16, P = static_cast<int>(a.head_dim), n_of = static_cast<int>(a.d_state);
+    const int n = 16 * w + c;
+    float phi[KS], psi[4];
+    const auto load = [&](size_t seg) {
+        const float *at = sg.carry + (bh * sg.count + seg) * (sg.cols + N) * N;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) psi[r] = at[(p0 + 4 * g + r) * N + n];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) phi[k] = at[(sg.cols + 4 * k + g) * N + n];
+    };
+    load(0);
+    for (int i = tid; i < 16 * N; i += 4 * N) {
+        const int p = p0 + i / N, m = i % N;
+        const float v = a.state && p < P && m < n_of ? a.state[(bh * P + p) * n_of + m] : 0.f;
+        s[0][i / N][m] = v;
+        sg.starts[(bh * sg.count * sg.cols + p) * N + m] = v;
+    }
+    scan::lds_barrier();
+    for (size_t seg = 0; seg + 1 < sg.count; ++seg) {
+        const float(*from)[N + 4] = s[seg & 1];
+        f32x4 acc[2] = {f32x4{psi[0], psi[1], psi[2], psi[3]}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        float m[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) m[k] = phi[k];
+        if (seg + 2 < sg.count) load(seg + 1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) acc[k & 1] = mfma_f32(from[c][4 * k + g], m[k], acc[k & 1]);
+        float *out = sg.starts + (bh * sg.count + seg + 1) * sg.cols * N;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float v = acc[0][r] + acc[1][r];
+            s[(seg + 1) & 1][4 * g + r][n] = v;
+            out[(p0 + 4 * g + r) * N + n] = v;
+        }
+        scan::lds_barrier();
+    }
+}
+
+// Segments of a window, by the time its chunk passes take in chunks (an LDS-full
+// workgroup a CU, 256 CUs; each segment joined 3/4 of a chunk, the launches four).  Measured on MI355X, one
+// sequence of 12 heads (64, 128), bf16, with and without: 16384 tokens 334 against 828 us, 2048
+// 77 against 116; from 24 heads of 2048 tokens on a window stays whole.
+size_t segments_of(const DeltaLaunch &a) {
+    const size_t chunks = chunks_of(a), heads = a.batch * a.heads, n = a.d_state <= 64 ? 64 : 128;
+    const size_t tiles = (a.head_dim + kCols - 1) / kCols;
+    const auto rounds = [](size_t wgs) { return (wgs + 255) / 256; };
+    size_t best = 1, least = rounds(heads * tiles) * chunks;
+    for (size_t count = 2; count <= 32 && count * 4 <= chunks; ++count) {
+        const size_t each = (chunks + count - 1) / count;
+        const size_t time = each * (rounds(heads * count * (tiles + n / kCols)) + rounds(heads * count * tiles)) + 4 + count * 3 / 4;
+        if (time < least) {
+            least = time;
+            best = count;
+        }
+    }
+    return best;
+}
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Where a call's segments lie in its workspace from byte `at` on.
+struct SegmentPlan {
+    size_t count, cols, n, carry, starts, bytes;
+    SegmentPlan(const DeltaLaunch &a, size_t at) : count(segments_of(a)), cols(Kept(a).p64), n(Kept(a).n) {
+        const size_t heads = a.batch * a.heads;
+        carry = align256(at);
+        starts = carry + (count > 1 ? heads * count * (cols + n) * n * sizeof(float) : 0);
+        bytes = starts + (count > 1 ? heads * count * cols * n * sizeof(float) : 0);
+    }
+};
+
+template <bool BACK>
+size_t record_units(const DeltaLaunch &a) {
+    size_t units = BackRecord::units;
+    if (!BACK)
+        (void)by_type(a.dtype, [&](auto t) {
+            units = Record<decltype(t)>::units;
+            return hipSuccess;
+        });
+    return units;
+}
+template <bool BACK>
+size_t records_bytes(const DeltaLaunch &a) {
+    return align256(a.batch * a.heads * chunks_of(a) * record_units<BACK>(a) * 1024);
+}
+
+// delta_prep, the segments' states where there is more than one, and the window's
+// pass (BACK: the backward's way in).
+template <bool BACK>
+hipError_t launch(const DeltaLaunch &a, unsigned char *workspace, size_t segments_at, float *kept, hipStream_t s,
+                  int &launches) {
     return by_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         return by_state(a.d_state, [&](auto n) {
-            constexpr int N = decltype(n)::value;
+            constexpr int N = decltype(n)::value, MODE = BACK ? kKeep : kWindow;
             const int chunks = static_cast<int>(chunks_of(a));
-            const dim3 prep(static_cast<unsigned>(a.batch * a.heads * chunks));
-            const dim3 main(static_cast<unsigned>(a.batch * a.heads), static_cast<unsigned>(KEEP ? kept_cols(a) : (a.head_dim + kCols - 1) / kCols));
+            const unsigned heads = static_cast<unsigned>(a.batch * a.heads);
+            const SegmentPlan plan(a, segments_at);
+            const Segments sg{plan.count, (chunks + static_cast<int>(plan.count) - 1) / static_cast<int>(plan.count),
+                              plan.cols, reinterpret_cast<float *>(workspace + plan.carry),
+                              reinterpret_cast<float *>(workspace + plan.starts)};
+            const unsigned tiles = static_cast<unsigned>(BACK ? kept_cols(a) : (a.head_dim + kCols - 1) / kCols);
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
-                hipLaunchKernelGGL((delta_prep<T, N, VEC, KEEP>), prep, dim3(256), 0, s, a, records, chunks);
-                hipLaunchKernelGGL((delta_chunks<T, N, VEC, KEEP>), main, dim3(256), 0, s, a, records, chunks, kept);
+                hipLaunchKernelGGL((delta_prep<T, N, VEC, BACK>), dim3(heads * chunks), dim3(256), 0, s, a, workspace,
+                                   chunks);
+                if (plan.count > 1) {
+                    const dim3 carry(heads * static_cast<unsigned>(plan.count),
+                                     static_cast<unsigned>((plan.cols + N) / kCols));
+                    hipLaunchKernelGGL((delta_chunks<T, N, VEC, kCarry, BACK>), carry, dim3(256), 0, s, a, workspace,
+                                       chunks, kept, sg);
+                    hipLaunchKernelGGL((delta_join<N>), dim3(heads, static_cast<unsigned>(plan.cols / 16)), dim3(4 * N), 0,
+                                       s, a, sg);
+                    launches += 2;
+                }
+                hipLaunchKernelGGL((delta_chunks<T, N, VEC, MODE, BACK>),
+                                   dim3(heads * static_cast<unsigned>(plan.count), tiles), dim3(256), 0, s, a,
+                                   workspace, chunks, kept, sg);
                 launches += 2;
                 return hipGetLastError();
             };
@@ -457,24 +637,31 @@ bool delta::rows_vec(const DeltaLaunch &a, size_t size) {
            ok(a.y, a.heads * a.head_dim);
 }
 
-hipError_t delta::launch_delta_states(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s,
-                                      int &launches) {
-    return launch<true>(a, records, kept, s, launches);
+size_t delta::delta_states_workspace(const DeltaLaunch &a, size_t &kept_at) {
+    const size_t records = records_bytes<true>(a);
+    kept_at = records;
+    return SegmentPlan(a, records + a.batch * a.heads * chunks_of(a) * Kept(a).floats() * sizeof(float)).bytes;
 }
 
-bool delta_chunk_wanted(const DeltaLaunch &a) { return a.d_state <= 128 && a.seq > 16; }
-
-size_t delta_chunk_workspace(const DeltaLaunch &a) {
-    size_t bytes = 0;
-    (void)by_type(a.dtype, [&](auto t) {
-        bytes = a.batch * a.heads * chunks_of(a) * Record<decltype(t)>::units * 1024;
-        return hipSuccess;
-    });
-    return bytes;
+hipError_t delta::launch_delta_states(const DeltaLaunch &a, unsigned char *workspace, hipStream_t s, int &launches) {
+    size_t kept_at = 0;
+    delta_states_workspace(a, kept_at);
+    return launch<true>(a, workspace, kept_at + a.batch * a.heads * chunks_of(a) * Kept(a).floats() * sizeof(float),
+                        reinterpret_cast<float *>(workspace + kept_at), s, launches);
 }
+
+// Against the recurrence token by token, which reads and writes the state once and
+// then takes its tokens one by one.  Measured on MI355X, heads of (64, 128) bf16,
+// recurrence and chunks: 96 heads 16 tokens 17.5 and 20 us a call, 8 tokens 16 and
+// 20; 1536 heads 16 tokens 65 and 120, growing by 3.4 a token against 0.3.
+bool delta_chunk_wanted(const DeltaLaunch &a) {
+    return a.d_state <= 128 && a.seq > (a.batch * a.heads >= 1024 ? 32u : 16u);
+}
+
+size_t delta_chunk_workspace(const DeltaLaunch &a) { return SegmentPlan(a, records_bytes<false>(a)).bytes; }
 
 hipError_t launch_delta_chunk(const DeltaLaunch &a, void *workspace, hipStream_t s, int &launches) {
-    return launch<false>(a, static_cast<unsigned char *>(workspace), nullptr, s, launches);
+    return launch<false>(a, static_cast<unsigned char *>(workspace), records_bytes<false>(a), nullptr, s, launches);
 }
 
 }  // namespace m3

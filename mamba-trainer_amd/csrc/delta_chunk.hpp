@@ -484,8 +484,19 @@ struct Kept {
 // The backward's chunk kernels write all of P64.
 inline size_t kept_cols(const DeltaLaunch &a) { return Kept(a).p64 / kCols; }
 
-// delta_prep and the forward states of the backward (delta_chunk.hip).
-hipError_t launch_delta_states(const DeltaLaunch &a, unsigned char *records, float *kept, hipStream_t s, int &launches);
+// A window's segments: how many, chunks of each, and where their states are, f32:
+// carry [heads][count][cols + N][N] (Psi, then Phi), starts [heads][count][cols][N].
+struct Segments {
+    size_t count;
+    int chunks;
+    size_t cols;
+    float *carry, *starts;
+};
+
+// delta_prep and the forward states of the backward (delta_chunk.hip): the
+// workspace of both, with the records first and what is kept from byte kept_at on.
+size_t delta_states_workspace(const DeltaLaunch &a, size_t &kept_at);
+hipError_t launch_delta_states(const DeltaLaunch &a, unsigned char *workspace, hipStream_t s, int &launches);
 
 }  // namespace delta
 }  // namespace m3

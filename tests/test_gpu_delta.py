@@ -350,3 +350,34 @@ def test_graph_replays_on_changed_inputs():
         torch.cuda.synchronize()
         for i, (a, b) in enumerate(zip(all_of(before), got)):
             assert torch.equal(a, b), (rep, i)
+
+
+@pytest.mark.parametrize("B,H,G,P,N,T,lengths,dtype", [
+    (1, 2, 2, 64, 128, 1500, None, BF), (2, 2, 1, 48, 96, 900, [900, 130], BF), (1, 1, 1, 16, 32, 2100, None, FL),
+    (1, 3, 3, 130, 64, 700, None, HF), (2, 1, 1, 7, 5, 600, [0, 600], FL)])
+def test_long_windows_of_few_heads(B, H, G, P, N, T, lengths, dtype):
+    """Windows that are cut into segments run side by side, sequences that end before the last of
+    them (or at once) among them; in place on the carried state as well."""
+    c = dc.make(T, B, T, H, G, P, N, dtype, lengths=lengths, decay=(1e-4, 1e-1))
+    check_forward(c)
+    check_backward(c)
+    c = dc.make(T, B, T, H, G, P, N, dtype, lengths=lengths, carried=False)
+    check_forward(c)
+
+
+def test_state_updated_in_place_by_a_window():
+    import ctypes as C
+    from mamba3 import _lib
+    L = _lib.lib()
+    for T in (5, 130, 800):
+        c = dc.make(T, 2, T, 2, 2, 64, 128, BF)
+        want_y, want_s = run(c)
+        s, y = c["h0"].clone(), torch.empty_like(c["v"])
+        cin = _lib.DeltaInputsC(2, T, 2, 2, 64, 128, _lib.M3_BF16, c["q"].data_ptr(), c["k"].data_ptr(),
+                                c["v"].data_ptr(), 0, 0, 0, c["g"].data_ptr(), c["beta"].data_ptr(), None,
+                                s.data_ptr(), 128 ** -0.5, 1, None, 0)
+        need = int(L.m3_delta_rule_workspace_bytes(C.byref(cin)))
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=DEV)
+        cin.workspace, cin.workspace_bytes = ws.data_ptr(), need
+        _lib.check(L.m3_delta_rule(C.byref(cin), y.data_ptr(), s.data_ptr(), _lib.stream_of(s)))
+        assert torch.equal(y, want_y) and torch.equal(s, want_s), T
