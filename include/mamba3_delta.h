@@ -51,6 +51,13 @@ typedef struct m3_delta_inputs {
     size_t workspace_bytes;
 } m3_delta_inputs;
 
+/* g and beta [rows, heads] from a projection's columns a and b (rows `stride`
+ * elements apart, of `dtype`): g = -exp(a_log[h]) softplus(a + dt_bias[h]), beta =
+ * sigmoid(b).  dt_bias [heads] may be NULL (zeros). */
+m3_status m3_delta_gates(size_t rows, size_t heads, int32_t dtype, const void *a, const void *b,
+                         size_t stride, const float *a_log, const float *dt_bias, float *g,
+                         float *beta, void *stream);
+
 /* The workspace of m3_delta_rule for these shapes; 0 where it needs none or
  * they are not covered. */
 size_t m3_delta_rule_workspace_bytes(const m3_delta_inputs *in);

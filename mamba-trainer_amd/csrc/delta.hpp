@@ -34,6 +34,10 @@ constexpr size_t kDeltaMaxState = 256;
 // The recurrence token by token with the state in registers (delta_recur.hip).
 hipError_t launch_delta_recur(const DeltaLaunch &a, hipStream_t s);
 
+// g and beta from a projection's columns (delta_recur.hip).
+hipError_t launch_delta_gates(size_t rows, size_t heads, int dtype, const void *pa, const void *pb, size_t stride,
+                              const float *a_log, const float *dt_bias, float *g, float *beta, hipStream_t s);
+
 // Chunk by chunk on the MFMA (delta_chunk.hip): whether a window takes this
 // form, the workspace it needs, and the launch.
 bool delta_chunk_wanted(const DeltaLaunch &a);

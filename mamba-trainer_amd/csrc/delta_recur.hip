@@ -176,6 +176,21 @@ __global__ void __launch_bounds__(TH) delta_recur_kernel(DeltaLaunch a) {
     }
 }
 
+// One thread a (row, head): a few bytes each, bound by the launch.
+template <typename T>
+__global__ void __launch_bounds__(256)
+delta_gates_kernel(size_t n, size_t heads, const T *pa, const T *pb, size_t stride, const float *a_log,
+                   const float *dt_bias, float *g, float *beta) {
+    const size_t i = blockIdx.x * size_t(256) + threadIdx.x;
+    if (i >= n) return;
+    const size_t row = i / heads, h = i % heads;
+    const float x = ldf(pa + row * stride + h) + (dt_bias ? dt_bias[h] : 0.f);
+    // softplus: x + log(1 + exp(-x)) where exp(x) could overflow
+    const float sp = (x > 0.f ? x : 0.f) + log1pf(expf(-fabsf(x)));
+    g[i] = -expf(a_log[h]) * sp;
+    beta[i] = 1.0f / (1.0f + expf(-ldf(pb + row * stride + h)));
+}
+
 template <typename T, int CH, int RPL, int TH>
 hipError_t go(const DeltaLaunch &a, hipStream_t s) {
     const auto ok = [](const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; };
@@ -200,6 +215,19 @@ hipError_t by_rows(const DeltaLaunch &a, hipStream_t s) {
 }
 
 }  // namespace
+
+hipError_t launch_delta_gates(size_t rows, size_t heads, int dtype, const void *pa, const void *pb, size_t stride,
+                              const float *a_log, const float *dt_bias, float *g, float *beta, hipStream_t s) {
+    const size_t n = rows * heads;
+    if (n == 0) return hipSuccess;
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(delta_gates_kernel<T>, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, n,
+                           heads, static_cast<const T *>(pa), static_cast<const T *>(pb), stride, a_log, dt_bias, g,
+                           beta);
+        return hipGetLastError();
+    });
+}
 
 hipError_t launch_delta_recur(const DeltaLaunch &a, hipStream_t s) {
     if (a.batch == 0) return hipSuccess;

@@ -81,6 +81,25 @@ m3_status check_workspace(const m3_delta_inputs *in, size_t need) {
 
 extern "C" {
 
+m3_status m3_delta_gates(size_t rows, size_t heads, int32_t dtype, const void *a, const void *b, size_t stride,
+                         const float *a_log, const float *dt_bias, float *g, float *beta, void *stream) {
+    if (dtype != M3_F32 && dtype != M3_BF16 && dtype != M3_F16)
+        return m3::api_fail(M3_ERR_ARGUMENT, "unknown dtype %d", static_cast<int>(dtype));
+    if (heads == 0) return m3::api_fail(M3_ERR_CONFIG, "delta rule dimensions must all be positive");
+    if (stride < heads)
+        return m3::api_fail(M3_ERR_SHAPE, "rows (%zu apart) are shorter than the heads (%zu)", stride, heads);
+    if (product_over(rows, heads, kMost))
+        return m3::api_fail(M3_ERR_UNSUPPORTED, "rows x heads must stay below 2^31 (got %zu x %zu)", rows, heads);
+    if (rows == 0) return m3::api_ok();
+    if (a == nullptr || b == nullptr || a_log == nullptr || g == nullptr || beta == nullptr)
+        return m3::api_fail(M3_ERR_ARGUMENT, "a, b, a_log, g and beta are required");
+    const hipError_t e = m3::launch_delta_gates(rows, heads, dtype, a, b, stride, a_log, dt_bias, g, beta,
+                                                as_stream(stream));
+    if (e != hipSuccess) return m3::api_hip_fail(e, "delta gates launch");
+    m3::count_launches(1);
+    return m3::api_ok();
+}
+
 size_t m3_delta_rule_workspace_bytes(const m3_delta_inputs *in) {
     if (check(in) != M3_OK || in->batch == 0) return 0;
     const m3::DeltaLaunch a = launch_of(in);

@@ -7,6 +7,7 @@ C ABI of libmamba3_hip.so (include/mamba3_ssm.h).
 from . import _lib
 from .error import (ArgumentError, ConfigError, DeviceError, Mamba3Error, RankError, ShapeError,
                     UnsupportedError)
+from .delta import GatedDeltaConfig, GatedDeltaMixer, GatedDeltaStack
 from .infer import StateCache
 from .ssm import (Discretization, ScanInputs, ScanOutput, SsmConfig, SsmMode, SsmState,
                   StateDynamics, mamba3_scan, mamba3_step, mamba3_step_, shift_left, ssd_chunked)

@@ -175,6 +175,7 @@ SIGNATURES = {
     "m3_block_norm_backward_workspace_bytes": (_Z, [C.POINTER(BlockNormC)]),
     "m3_block_norm_backward": (C.c_int, [C.POINTER(BlockNormC), C.POINTER(BlockNormGradsC), _P, _Z, _P]),
     # mamba3_delta.h
+    "m3_delta_gates": (C.c_int, [_Z, _Z, C.c_int32, _P, _P, _Z] + [_P] * 5),
     "m3_delta_rule_workspace_bytes": (_Z, [C.POINTER(DeltaInputsC)]),
     "m3_delta_rule": (C.c_int, [C.POINTER(DeltaInputsC), _P, _P, _P]),
     "m3_delta_step": (C.c_int, [C.POINTER(DeltaInputsC), _P, _P, _P]),

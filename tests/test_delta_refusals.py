@@ -42,6 +42,18 @@ def test_delta_rule_refusals(kw, status, message):
     assert L.m3_launch_count() == before
 
 
+def test_delta_gates_refusals():
+    from mamba3 import _lib
+    L = _lib.lib()
+    call = lambda rows, heads, dt, stride, a: L.m3_delta_gates(rows, heads, dt, a, FAKE, stride, FAKE, None, FAKE, FAKE, None)
+    assert call(4, 0, 1, 8, FAKE) == _lib.M3_ERR_CONFIG
+    assert call(4, 4, 5, 8, FAKE) == _lib.M3_ERR_ARGUMENT
+    assert call(4, 9, 1, 8, FAKE) == _lib.M3_ERR_SHAPE
+    assert call(1 << 31, 4, 1, 8, FAKE) == _lib.M3_ERR_UNSUPPORTED
+    assert call(4, 4, 1, 8, None) == _lib.M3_ERR_ARGUMENT
+    assert call(0, 4, 1, 8, None) == _lib.M3_OK
+
+
 def test_delta_rule_buffers():
     from mamba3 import _lib
     L = _lib.lib()
