@@ -73,6 +73,20 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             in.fetch(live - 1);
         }
     }
+    // rows 32 half .. of a chunk's dR: written a chunk later, so that the wait for
+    // the operands does not wait for them
+    f32x4 late[2];
+    const auto write = [&](int ck) {
+        float *keep = kept + (bh * chunks + ck) * kd.floats();
+        const Rows<T, VEC> dvr(dvp + static_cast<size_t>(ck) * kC * pv, pv, len - ck * kC, P);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                keep[kd.dr() + (32 * half + 16 * i + 4 * g + r) * kd.p64 + p] = late[i][r];
+                store_one(dvr, dv_at, 4 * g, p, 32 * half + 16 * i + r, late[i][r]);
+            }
+    };
     for (int ck = live - 1; ck >= 0; --ck) {
         const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
         const typename St::Rows1 &k = sk[now], &q1 = sq[now];
@@ -88,6 +102,7 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             __syncthreads();
             if (ck > 0) in.fetch(ck - 1);
         }
+        if (ck + 1 < live) write(ck + 1);
         float *keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -161,20 +176,14 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
                 }
         };
         cols(0);
-        // x is dR: rows 32 half .. are this wave's to write
-        const Rows<T, VEC> dvr(dvp + static_cast<size_t>(ck) * kC * pv, pv, len - ck * kC, P);
+        // x is dR
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v;
-                if (half)
-                    v = x[2 + i][r];
-                else
-                    v = x[i][r];
-                keep[kd.dr() + (32 * half + 16 * i + 4 * g + r) * kd.p64 + p] = v;
-                store_one(dvr, dv_at, 4 * g, p, 32 * half + 16 * i + r, v);
-            }
+        for (int i = 0; i < 2; ++i) {
+            if (half)
+                late[i] = x[2 + i];
+            else
+                late[i] = x[i];
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] *= -*reinterpret_cast<const f32x4 *>(fac + kFacK + 16 * i + 4 * g);
@@ -196,6 +205,7 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (live > 0) write(0);
     if (p >= P) return;
     if (half == 0)
         for (int t = len + g; t < L; t += 4) stf(dvp + t * pv + p, 0.f);

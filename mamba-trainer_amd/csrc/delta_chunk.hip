@@ -304,6 +304,37 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             in.fetch(first);
         }
     }
+    // rows 32 half .. of a chunk's Y (KEEP: E): written a chunk later, so that the
+    // wait for the operands does not wait for them
+    f32x4 late[2];
+    const auto write = [&](int ck) {
+        if constexpr (KEEP) {
+            float *to = kept + (bh * chunks + ck) * kd.floats() + kd.e() + (32 * half + 4 * g) * kd.p64 + p;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[(16 * i + r) * kd.p64] = late[i][r];
+        }
+        if constexpr (Y) {
+            // padding rows past the buffer's end are dropped
+            const Rows<T, VEC> yrow(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
+            if constexpr (DMA) {
+                // the wave's 32 x 16 through LDS to 16-byte stores
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        sy[wave][16 * i + 4 * g + r][c] = from_f32<bf16_t>(late[i][r]).bits;
+                bst16(*reinterpret_cast<const u32x4 *>(&sy[wave][lane >> 1][8 * (lane & 1)]), yrow.r,
+                      row_off<T>(ystep, P, 32 * half + (lane >> 1), p0 + 16 * w + 8 * (lane & 1)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) store_one(yrow, y_at, 4 * g, p, 32 * half + 16 * i + r, late[i][r]);
+            }
+        }
+    };
     for (int ck = first; ck < live; ++ck) {
         const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
         const typename St::Rows1 &k = sk[now];
@@ -319,9 +350,9 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             __syncthreads();
             if (ck + 1 < live) in.fetch(ck + 1);
         }
-        float *keep = nullptr;
+        if (ck > first) write(ck - 1);
         if constexpr (KEEP) {
-            keep = kept + (bh * chunks + ck) * kd.floats();
+            float *keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 *reinterpret_cast<f32x4 *>(keep + kd.s0() + p * N + state_n(nt0 + nt, g, 0)) = S[nt];
@@ -408,15 +439,12 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         cols(0);
         if constexpr (KEEP) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float *to = keep + kd.e() + (32 * half + 16 * i + 4 * g + r) * kd.p64 + p;
-                    if (half)
-                        *to = e[2 + i][r];
-                    else
-                        *to = e[i][r];
-                }
+            for (int i = 0; i < 2; ++i) {
+                if (half)
+                    late[i] = e[2 + i];
+                else
+                    late[i] = e[i];
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -453,24 +481,10 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         if constexpr (!Y) continue;
         mma_rows<2, YP, YP>(pb[0], xe[0], yr);
         if (half) mma_rows<2, YP, YP>(pb[1], xe[1], yr);
-        // padding rows past the buffer's end are dropped
-        const Rows<T, VEC> yrow(yp + static_cast<size_t>(ck) * kC * ystep, ystep, len - ck * kC, P);
-        if constexpr (DMA && Y) {
-            // the wave's 32 x 16 through LDS to 16-byte stores
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    sy[wave][16 * i + 4 * g + r][c] = from_f32<bf16_t>(yr[i][r]).bits;
-            bst16(*reinterpret_cast<const u32x4 *>(&sy[wave][lane >> 1][8 * (lane & 1)]), yrow.r,
-                  row_off<T>(ystep, P, 32 * half + (lane >> 1), p0 + 16 * w + 8 * (lane & 1)));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) store_one(yrow, y_at, 4 * g, p, 32 * half + 16 * i + r, yr[i][r]);
-        }
+        late[0] = yr[0];
+        late[1] = yr[1];
     }
+    if (first < live) write(live - 1);
     if constexpr (MODE == kCarry) {
         float *to = sg.carry + ((bh * sg.count + seg) * (sg.cols + N) + p) * N;
 #pragma unroll
