@@ -31,7 +31,7 @@ using namespace delta;
 // the first, in pairs of waves as delta_chunks: a wave has half of N of its
 // sixteen columns of the state's gradient.
 template <typename T, int N, bool VEC>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ void __launch_bounds__((kChunkThreads<T, VEC>))
 delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chunks, float *kept) {
     constexpr int KP = Parts<T>::in, KS = N / 64, NT = N / 32;   // of this wave
     using St = Stage<T, N, VEC, true, 1 + 2 * kTriT, kTriT>;
@@ -63,15 +63,28 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         }
     const int live = (len + kC - 1) / kC;
     St in(a, b, h, len, static_cast<const T *>(gr.dy) + row0, pv, p0, records + bh * chunks * rec_bytes, rec_bytes);
-    if (live > 0) {
-        if constexpr (DMA) {
-            in.dma_k(sk[(live - 1) & 1], live - 1);
-            in.dma_q(sq[(live - 1) & 1], live - 1);
-            in.dma_v(sv, live - 1);
-            in.dma_rec(sr[(live - 1) & 1], live - 1);
-        } else {
-            in.fetch(live - 1);
+    if constexpr (DMA) {
+        if (wave == 4) {
+            const auto bring = [&](int ck) {
+                in.dma_k(sk[ck & 1], ck);
+                in.dma_q(sq[ck & 1], ck);
+                in.dma_rec(sr[ck & 1], ck);
+            };
+            if (live > 0) {
+                bring(live - 1);
+                in.dma_v(sv, live - 1);
+            }
+            for (int ck = live - 1; ck >= 0; --ck) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                scan::lds_barrier();   // the chunk is there, the one after it is done with
+                if (ck > 0) bring(ck - 1);
+                scan::lds_barrier();   // dY is done with
+                if (ck > 0) in.dma_v(sv, ck - 1);
+            }
+            return;
         }
+    } else {
+        if (live > 0) in.fetch(live - 1);
     }
     // rows 32 half .. of a chunk's dR: written a chunk later, so that the wait for
     // the operands does not wait for them
@@ -88,13 +101,12 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             }
     };
     for (int ck = live - 1; ck >= 0; --ck) {
-        const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
+        const int now = DMA ? ck & 1 : 0;
         const typename St::Rows1 &k = sk[now], &q1 = sq[now];
         const unsigned char *rec = sr[now].at;
         f32x4 dy[4];
         if constexpr (DMA) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            scan::lds_barrier();
         } else {
             __syncthreads();
             in.put(sk[0], sq[0], sr[0]);
@@ -128,8 +140,6 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
                 tri_load<kNP>(rec + (1 + kTriT) * 1024, lane, p4, p2, true);
                 if constexpr (DMA) in.values(sv, dy);
             }
-            if constexpr (DMA)
-                if (ck > 0 && kk == 0) in.dma_k(sk[nxt], ck - 1);
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
@@ -147,12 +157,6 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         }
         tri_load<kNP>(rec + 1024, lane, t4, t2, true);
         scan::lds_barrier();
-        if constexpr (DMA)
-            if (ck > 0) {
-                in.dma_q(sq[nxt], ck - 1);
-                in.dma_v(sv, ck - 1);
-                in.dma_rec(sr[nxt], ck - 1);
-            }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             ks[i] += meet[wave ^ 1][i][lane];
@@ -686,7 +690,8 @@ hipError_t launch_delta_backward(const DeltaLaunch &a, const DeltaGrads &g, void
             const dim3 own(static_cast<unsigned>(a.batch * a.groups * chunks));
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
-                hipLaunchKernelGGL((delta_reverse<T, N, VEC>), rev, dim3(256), 0, s, a, g, records, chunks, kept);
+                constexpr unsigned threads = kChunkThreads<T, VEC>;
+                hipLaunchKernelGGL((delta_reverse<T, N, VEC>), rev, dim3(threads), 0, s, a, g, records, chunks, kept);
                 ++launches;
                 if (chunks > 0) {
                     if (a.heads == a.groups)

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // (2 P + N) / P times the work, in segments' time.
 enum { kWindow, kKeep, kCarry };
 template <typename T, int N, bool VEC, int MODE, bool BACK>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ void __launch_bounds__((kChunkThreads<T, VEC>))
 delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept, Segments sg) {
     constexpr bool KEEP = MODE == kKeep, Y = MODE == kWindow;
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 64, NT = N / 32;   // of this wave
@@ -294,15 +294,29 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
     const int live = sg.chunks < all - first ? first + sg.chunks : all;   // the segment's end
     St in(a, b, h, len, static_cast<const T *>(a.v) + b * L * a.vs + h * P, a.vs, p0,
           records + bh * chunks * rec_bytes, rec_bytes);
-    if (first < live) {
-        if constexpr (DMA) {
-            in.dma_k(sk[first & 1], first);
-            if constexpr (Y) in.dma_q(sq, first);
-            in.dma_v(sv[first & 1], first);
-            in.dma_rec(sr[first & 1], first);
-        } else {
-            in.fetch(first);
+    if constexpr (DMA) {
+        if (wave == 4) {
+            const auto bring = [&](int ck) {
+                in.dma_k(sk[ck & 1], ck);
+                in.dma_v(sv[ck & 1], ck);
+                in.dma_rec(sr[ck & 1], ck);
+            };
+            if (first < live) {
+                bring(first);
+                if constexpr (Y) in.dma_q(sq, first);
+            }
+            for (int ck = first; ck < live; ++ck) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                scan::lds_barrier();   // the chunk is there, the one before is done with
+                if (ck + 1 < live) bring(ck + 1);
+                scan::lds_barrier();   // Q is done with
+                if constexpr (Y)
+                    if (ck + 1 < live) in.dma_q(sq, ck + 1);
+            }
+            return;
         }
+    } else {
+        if (first < live) in.fetch(first);
     }
     // rows 32 half .. of a chunk's Y (KEEP: E): written a chunk later, so that the
     // wait for the operands does not wait for them
@@ -336,13 +350,12 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         }
     };
     for (int ck = first; ck < live; ++ck) {
-        const int now = DMA ? ck & 1 : 0, nxt = DMA ? (ck + 1) & 1 : 0;
+        const int now = DMA ? ck & 1 : 0;
         const typename St::Rows1 &k = sk[now];
         const unsigned char *rec = sr[now].at;
         f32x4 e[4];
         if constexpr (DMA) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            scan::lds_barrier();
         } else {
             __syncthreads();
             in.put(sk[0], sq, sr[0]);
@@ -383,11 +396,6 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             } else {
                 if constexpr (DMA) in.values(sv[now], e);
             }
-            if constexpr (DMA)
-                if (ck + 1 < live && kk == 0) {
-                    in.dma_k(sk[nxt], ck + 1);
-                    in.dma_v(sv[nxt], ck + 1);
-                }
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
@@ -413,11 +421,6 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             ks[i] += meet[wave ^ 1][i][lane];
             e[i] -= *reinterpret_cast<const f32x4 *>(fac + kFacK + 16 * i + 4 * g) * ks[i];
         }
-        if constexpr (DMA)
-            if (ck + 1 < live) {
-                if constexpr (Y) in.dma_q(sq, ck + 1);
-                in.dma_rec(sr[nxt], ck + 1);
-            }
         // E = T R
         bf16x8 x[2][kNP];
         split_tiles<kNP>(e[0], e[1], x[0]);
@@ -616,19 +619,20 @@ hipError_t launch(const DeltaLaunch &a, unsigned char *workspace, size_t segment
             const unsigned tiles = static_cast<unsigned>(BACK ? kept_cols(a) : (a.head_dim + kCols - 1) / kCols);
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
+                constexpr unsigned threads = kChunkThreads<T, VEC>;
                 hipLaunchKernelGGL((delta_prep<T, N, VEC, BACK>), dim3(heads * chunks), dim3(256), 0, s, a, workspace,
                                    chunks);
                 if (plan.count > 1) {
                     const dim3 carry(heads * static_cast<unsigned>(plan.count),
                                      static_cast<unsigned>((plan.cols + N) / kCols));
-                    hipLaunchKernelGGL((delta_chunks<T, N, VEC, kCarry, BACK>), carry, dim3(256), 0, s, a, workspace,
+                    hipLaunchKernelGGL((delta_chunks<T, N, VEC, kCarry, BACK>), carry, dim3(threads), 0, s, a, workspace,
                                        chunks, kept, sg);
                     hipLaunchKernelGGL((delta_join<N>), dim3(heads, static_cast<unsigned>(plan.cols / 16)), dim3(4 * N), 0,
                                        s, a, sg);
                     launches += 2;
                 }
                 hipLaunchKernelGGL((delta_chunks<T, N, VEC, MODE, BACK>),
-                                   dim3(heads * static_cast<unsigned>(plan.count), tiles), dim3(256), 0, s, a,
+                                   dim3(heads * static_cast<unsigned>(plan.count), tiles), dim3(threads), 0, s, a,
                                    workspace, chunks, kept, sg);
                 launches += 2;
                 return hipGetLastError();

@@ -318,12 +318,15 @@ constexpr int kCols = 32;
 
 // The fetch of a chunk's operands to LDS: K, Q, a tile of v (or dy), and UNITS
 // kilobytes of its record (unit u > 0 from kilobyte u + GAP).  bf16 with aligned
-// rows (DMA): straight from memory, piece by piece where the caller says.  Other
-// inputs become their bf16 parts on the way, through registers; v stays there.
+// rows (DMA): straight from memory, by a fifth wave that does nothing else (issuing
+// them stalls a wave some 100 cycles a kilobyte).  Other inputs become their bf16
+// parts on the way, through registers; v stays there.
+template <typename T, bool VEC> constexpr bool kDma = VEC && std::is_same<T, bf16_t>::value;
+template <typename T, bool VEC> constexpr unsigned kChunkThreads = kDma<T, VEC> ? 320 : 256;
 template <typename T, int N, bool VEC, bool WITHQ, int UNITS, int GAP>
 struct Stage {
     static constexpr int KP = Parts<T>::in;
-    static constexpr bool DMA = VEC && std::is_same<T, bf16_t>::value;
+    static constexpr bool DMA = kDma<T, VEC>;
     static constexpr int pieces = kC * N / 8 / 256, rpieces = UNITS / 4 + 1;
     struct Rows1 { unsigned char part[KP][Tile<N>::bytes]; };
     struct Rec { unsigned char at[UNITS * 1024]; };
@@ -331,8 +334,8 @@ struct Stage {
     const T *kp, *qp, *vp;              // the sequence's rows of this head
     size_t ks, qs, vs, rec_bytes;
     const unsigned char *rec;           // the sequence's records
-    int len, n_of, P, wave, w, lane;    // wave: of four; w: its tile of columns
-    uint32_t dk, dq, dv;                // DMA places
+    int len, n_of, P, wave, w, lane;    // wave: 4 is the DMA's; w: its tile of columns
+    uint32_t dk[4], dq[4], dv[4];       // DMA: places in a kilobyte, by kilobyte modulo 4
     int kt, kn, vt, vn;                 // else: this thread's places
     uint32_t k_at, q_at, v_at;
     Eight<T> k8[pieces], q8[WITHQ ? pieces : 1];
@@ -362,9 +365,12 @@ struct Stage {
         vt = 4 * (lane >> 4);
         vn = p0 + 16 * w + (lane & 15);
         if constexpr (DMA) {
-            dk = dma_at<T, N>(ks, n_of, 0, wave, lane);
-            dq = dma_at<T, N>(qs, n_of, 0, wave, lane);
-            dv = dma_at<T, kCols>(vs, P, p0, wave, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dk[i] = dma_at<T, N>(ks, n_of, 0, i, lane);
+                dq[i] = dma_at<T, N>(qs, n_of, 0, i, lane);
+                dv[i] = dma_at<T, kCols>(vs, P, p0, i, lane);
+            }
         } else {
             k_at = row_off<T>(ks, n_of, kt, kn);
             q_at = row_off<T>(qs, n_of, kt, kn);
@@ -377,16 +383,25 @@ struct Stage {
         return Rows<T, VEC>(p + static_cast<size_t>(ck) * kC * stride, stride, len - ck * kC, width);
     }
 
-    __device__ __forceinline__ void dma_k(Rows1 &to, int ck) const { dma_tile<N>(rows_of(kp, ks, ck, n_of), dk, to.part[0], wave); }
-    __device__ __forceinline__ void dma_q(Rows1 &to, int ck) const { dma_tile<N>(rows_of(qp, qs, ck, n_of), dq, to.part[0], wave); }
-    __device__ __forceinline__ void dma_v(V &to, int ck) const { dma_tile<kCols>(rows_of(vp, vs, ck, P), dv, to.at, wave); }
+    __device__ __forceinline__ void dma_k(Rows1 &to, int ck) const {
+        const Rows<T, VEC> rows = rows_of(kp, ks, ck, n_of);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dma_tile<N>(rows, dk[i], to.part[0], i);
+    }
+    __device__ __forceinline__ void dma_q(Rows1 &to, int ck) const {
+        const Rows<T, VEC> rows = rows_of(qp, qs, ck, n_of);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dma_tile<N>(rows, dq[i], to.part[0], i);
+    }
+    __device__ __forceinline__ void dma_v(V &to, int ck) const {
+        const Rows<T, VEC> rows = rows_of(vp, vs, ck, P);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dma_tile<kCols>(rows, dv[i], to.at, i);
+    }
     __device__ __forceinline__ void dma_rec(Rec &to, int ck) const {
         const rsrc_t r = record(ck);
 #pragma unroll
-        for (int i = 0; i < rpieces; ++i) {
-            const int u = wave + 4 * i;
-            if (u < UNITS) scan::lds_dma16(r, scan::lds_addr(to.at + u * 1024), unit(u) * 1024 + lane * 16);
-        }
+        for (int u = 0; u < UNITS; ++u) scan::lds_dma16(r, scan::lds_addr(to.at + u * 1024), unit(u) * 1024 + lane * 16);
     }
     __device__ __forceinline__ void fetch(int ck) {
         const Rows<T, VEC> kr = rows_of(kp, ks, ck, n_of), qr = rows_of(qp, qs, ck, n_of), vr = rows_of(vp, vs, ck, P);
