@@ -68,7 +68,7 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
             const auto bring = [&](int ck) {
                 in.dma_k(sk[ck & 1], ck);
                 in.dma_q(sq[ck & 1], ck);
-                in.dma_rec(sr[ck & 1], ck);
+                in.template dma_rec<0, 1 + 2 * kTriT>(sr[ck & 1].at, ck);
             };
             if (live > 0) {
                 bring(live - 1);
@@ -118,7 +118,7 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
         float *keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<f32x4 *>(keep + kd.s1() + p * N + state_n(nt0 + nt, g, 0)) = S[nt];
+            *reinterpret_cast<f32x4 *>(keep + kd.s1() + kd.tile(p, nt0 + nt, lane)) = S[nt];
         const float *fac = reinterpret_cast<const float *>(rec);
         f32x4 ks[4], x[4];
 #pragma unroll
@@ -388,15 +388,16 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
         }
         // what the states' first block takes, on its way during the triangle
         constexpr int pieces = 32 * N / 8 / 256;
-        const int pr = tid / per, pn = tid % per * 8;
+        // piece i of this wave: columns 16 (w & 1) .. of the block, n of the pair of tiles i
+        const auto pair = [&](int i) { return (w >> 1) + 2 * i; };
         f32x4 s0[pieces][2], s1[pieces][2], r1[2], e1[2];
         uint32_t y1[8];
         const auto load_state = [&](size_t at, int pb, f32x4(*out)[2]) {
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
-                const float *s = keep + at + (pb + pr + i * (256 / per)) * N + pn;
+                const float *s = keep + at + kd.tile(pb + 16 * (w & 1), 2 * pair(i), lane);
                 out[i][0] = *reinterpret_cast<const f32x4 *>(s);
-                out[i][1] = *reinterpret_cast<const f32x4 *>(s + 4);
+                out[i][1] = *reinterpret_cast<const f32x4 *>(s + 256);
             }
         };
         const auto load_first = [&](int pb) {
@@ -475,7 +476,7 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
 #pragma unroll
                     for (int q = 0; q < kNP; ++q)
                         *reinterpret_cast<bf16x8 *>(area + q * (Tile<N>::bytes / 2) +
-                                                    tile_at<N>(pr + i * (256 / per), pn / 8)) = x[q];
+                                                    tile_at<N>(16 * (w & 1) + c, 4 * pair(i) + g)) = x[q];
                 }
             };
             const auto state = [&](int nt, bf16x8 *out) {

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // (2 P + N) / P times the work, in segments' time.
 enum { kWindow, kKeep, kCarry };
 template <typename T, int N, bool VEC, int MODE, bool BACK>
-__global__ void __launch_bounds__((kChunkThreads<T, VEC>))
+__global__ void __launch_bounds__((kChunkThreads<T, VEC>), (kDma<T, VEC> && MODE != kWindow ? 3 : 1))
 delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept, Segments sg) {
     constexpr bool KEEP = MODE == kKeep, Y = MODE == kWindow;
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 64, NT = N / 32;   // of this wave
@@ -258,8 +258,10 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
     constexpr bool DMA = St::DMA;
     constexpr int BUFS = DMA ? 2 : 1;
     __shared__ __attribute__((aligned(1024))) typename St::Rows1 sk[BUFS];
-    __shared__ __attribute__((aligned(1024))) typename St::Rec sr[BUFS];
-    __shared__ __attribute__((aligned(1024))) typename St::V sv[BUFS];
+    constexpr bool TWO = DMA && Y;   // else only K and the record's factors lie there twice
+    __shared__ __attribute__((aligned(1024))) typename St::Rec sr[TWO ? 2 : 1];
+    __shared__ __attribute__((aligned(1024))) typename St::V sv[TWO ? 2 : 1];
+    __shared__ __attribute__((aligned(1024))) unsigned char odd_fac[DMA && !Y ? 1024 : 16];
     __shared__ __attribute__((aligned(1024))) unsigned char sq_[!Y ? 16 : sizeof(typename St::Rows1)];
     __shared__ f32x4 meet[4][Y ? 6 : 4][64];
     __shared__ __attribute__((aligned(16))) uint16_t sy[DMA && Y ? 4 : 1][DMA && Y ? 32 : 1][16];
@@ -296,22 +298,33 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
           records + bh * chunks * rec_bytes, rec_bytes);
     if constexpr (DMA) {
         if (wave == 4) {
-            const auto bring = [&](int ck) {
+            const auto first_half = [&](int ck) {
                 in.dma_k(sk[ck & 1], ck);
-                in.dma_v(sv[ck & 1], ck);
-                in.dma_rec(sr[ck & 1], ck);
+                if constexpr (Y) {
+                    in.dma_v(sv[ck & 1], ck);
+                    in.template dma_rec<0, R::units>(sr[ck & 1].at, ck);
+                } else {
+                    in.template dma_rec<0, 1>(ck & 1 ? odd_fac : sr[0].at, ck);
+                }
+            };
+            const auto second_half = [&](int ck) {
+                if constexpr (Y) {
+                    in.dma_q(sq, ck);
+                } else {
+                    in.dma_v(sv[0], ck);
+                    in.template dma_rec<R::t, R::p>(sr[0].at, ck);
+                }
             };
             if (first < live) {
-                bring(first);
-                if constexpr (Y) in.dma_q(sq, first);
+                first_half(first);
+                second_half(first);
             }
             for (int ck = first; ck < live; ++ck) {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 scan::lds_barrier();   // the chunk is there, the one before is done with
-                if (ck + 1 < live) bring(ck + 1);
-                scan::lds_barrier();   // Q is done with
-                if constexpr (Y)
-                    if (ck + 1 < live) in.dma_q(sq, ck + 1);
+                if (ck + 1 < live) first_half(ck + 1);
+                scan::lds_barrier();   // Q, or v and T, are done with
+                if (ck + 1 < live) second_half(ck + 1);
             }
             return;
         }
@@ -352,7 +365,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
     for (int ck = first; ck < live; ++ck) {
         const int now = DMA ? ck & 1 : 0;
         const typename St::Rows1 &k = sk[now];
-        const unsigned char *rec = sr[now].at;
+        const unsigned char *rec = sr[TWO ? now : 0].at;
         f32x4 e[4];
         if constexpr (DMA) {
             scan::lds_barrier();
@@ -368,9 +381,9 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             float *keep = kept + (bh * chunks + ck) * kd.floats();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                *reinterpret_cast<f32x4 *>(keep + kd.s0() + p * N + state_n(nt0 + nt, g, 0)) = S[nt];
+                *reinterpret_cast<f32x4 *>(keep + kd.s0() + kd.tile(p, nt0 + nt, lane)) = S[nt];
         }
-        const float *fac = reinterpret_cast<const float *>(rec);
+        const float *fac = reinterpret_cast<const float *>(DMA && !Y && now ? odd_fac : rec);
         // this half of K S0^T and Q S0^T: while a k-step is multiplied, the next
         // one's operands are read and its columns of S are split
         f32x4 y[4], ks[4];
@@ -394,7 +407,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             if (kk + 1 < KS) {
                 rows(kk + 1);
             } else {
-                if constexpr (DMA) in.values(sv[now], e);
+                if constexpr (DMA) in.values(sv[TWO ? now : 0], e);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);

@@ -398,10 +398,11 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < 4; ++i) dma_tile<kCols>(rows, dv[i], to.at, i);
     }
-    __device__ __forceinline__ void dma_rec(Rec &to, int ck) const {
+    template <int FROM, int END>   // kilobytes FROM .. of the record, to where its first would lie at `to`
+    __device__ __forceinline__ void dma_rec(unsigned char *to, int ck) const {
         const rsrc_t r = record(ck);
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) scan::lds_dma16(r, scan::lds_addr(to.at + u * 1024), unit(u) * 1024 + lane * 16);
+        for (int u = FROM; u < END; ++u) scan::lds_dma16(r, scan::lds_addr(to + u * 1024), unit(u) * 1024 + lane * 16);
     }
     __device__ __forceinline__ void fetch(int ck) {
         const Rows<T, VEC> kr = rows_of(kp, ks, ck, n_of), qr = rows_of(qp, qs, ck, n_of), vr = rows_of(vp, vs, ck, P);
@@ -485,10 +486,16 @@ hipError_t by_state(size_t d_state, F f) {
 
 // What the backward keeps of each chunk of a head, f32: the state before it and
 // the gradient of the state after it [P64][N] (P64: head_dim to the next multiple
-// of 64, N: 64 or 128), E and dR [64][P64].
+// of 64, N: 64 or 128) as the accumulators hold them, tile by tile of 16 columns
+// and 16 of N, a lane's four together, so that a wave's store is one kilobyte; E
+// and dR [64][P64].
 struct Kept {
     size_t p64, n;
     __host__ __device__ Kept(const DeltaLaunch &a) : p64((a.head_dim + 63) / 64 * 64), n(a.d_state <= 64 ? 64 : 128) {}
+    // a lane's part of tile nt of columns p ..
+    __device__ __forceinline__ size_t tile(int p, int nt, int lane) const {
+        return ((p / 16) * (n / 16) + nt) * 256 + 4 * lane;
+    }
     __host__ __device__ size_t s0() const { return 0; }
     __host__ __device__ size_t s1() const { return p64 * n; }
     __host__ __device__ size_t e() const { return 2 * p64 * n; }
