@@ -280,38 +280,39 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
     const Kept kd(a);
     const int my = 16 * w + c;
     // the group's rows, and the factors that bring them to unit length
+    constexpr int own_rows = kC * per / 256;
+    Eight<T> k8[own_rows], q8[own_rows];
     {
         const Rows<T, VEC> kr(static_cast<const T *>(a.k) + tok * a.ks + kg * n_of, a.ks, live, n_of);
         const Rows<T, VEC> qr(static_cast<const T *>(a.q) + tok * a.qs + kg * n_of, a.qs, live, n_of);
 #pragma unroll
-        for (int i = 0; i < kC * per / 256; ++i) {
-            const int t = tid / per + i * (256 / per), n = tid % per * 8;
-            const Eight<T> k8 = load_eight(kr, t, n), q8 = load_eight(qr, t, n);
-            float f[8], ssk = 0.f, ssq = 0.f;
-            widen(k8, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ssk += f[j] * f[j];
-            widen(q8, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ssq += f[j] * f[j];
-#pragma unroll
-            for (int off = 1; off < per; off <<= 1) {
-                ssk += __shfl_xor(ssk, off, 64);
-                ssq += __shfl_xor(ssq, off, 64);
-            }
-            if (n == 0) {
-                rk[t] = a.qk_norm ? 1.0f / sqrtf(ssk + kUnitEps) : 1.0f;
-                rq[t] = a.qk_norm ? 1.0f / sqrtf(ssq + kUnitEps) : 1.0f;
-            }
-            bf16x8 x[KP];
-            to_parts(k8, x);
-#pragma unroll
-            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(sk[q] + tile_at<N>(t, n / 8)) = x[q];
-            to_parts(q8, x);
-#pragma unroll
-            for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(sq[q] + tile_at<N>(t, n / 8)) = x[q];
+        for (int i = 0; i < own_rows; ++i) {
+            k8[i] = load_eight(kr, tid / per + i * (256 / per), tid % per * 8);
+            q8[i] = load_eight(qr, tid / per + i * (256 / per), tid % per * 8);
         }
     }
+    const auto put_row = [&](const Eight<T> &x8, unsigned char(*to)[Tile<N>::bytes], float *unit, int t) {
+        const int n = tid % per * 8;
+        float f[8], ss = 0.f;
+        widen(x8, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+#pragma unroll
+        for (int off = 1; off < per; off <<= 1) ss += __shfl_xor(ss, off, 64);
+        if (n == 0) unit[t] = a.qk_norm ? 1.0f / sqrtf(ss + kUnitEps) : 1.0f;
+        bf16x8 x[KP];
+        to_parts(x8, x);
+#pragma unroll
+        for (int q = 0; q < KP; ++q) *reinterpret_cast<bf16x8 *>(to[q] + tile_at<N>(t, n / 8)) = x[q];
+    };
+    const auto put_rows = [&]() {
+#pragma unroll
+        for (int i = 0; i < own_rows; ++i) {
+            put_row(k8[i], sk, rk, tid / per + i * (256 / per));
+            put_row(q8[i], sq, rq, tid / per + i * (256 / per));
+        }
+    };
+    if constexpr (MANY) put_rows();
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     // q (or k) at row r, column state_n(nt, c >> 2, c & 3), from its parts
     const int own = (16 * w + 4 * g) * (2 * N) + ((g ^ (c >> 2)) << 4) + 2 * (c & 3);
@@ -349,14 +350,15 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             for (int j = 0; j < 8; ++j) y8[j] = value_of<T>(y[j]);
             split8<KP>(y8, out);
         };
-        if (w == 0) {
-            const size_t th = (tok + lane) * a.heads + h;
-            G[lane] = wave_scan<1>(lane < live ? static_cast<double>(clamp_decay(a.g[th])) : 0.0, lane);
-            beta[lane] = lane < live ? a.beta[th] : 0.f;
+        // this head's decays, steps and factors, on their way while the rows are put down
+        const size_t th = (tok + lane) * a.heads + h;
+        float g1 = 0.f, b1 = 0.f;
+        f32x4 fac1 = zero;
+        if (w == 0 && lane < live) {
+            g1 = a.g[th];
+            b1 = a.beta[th];
         }
-        if (w == 1)
-            *reinterpret_cast<f32x4 *>(fac + 4 * lane) =
-                *reinterpret_cast<const f32x4 *>(records + rec * (BackRecord::units * 1024) + 16 * lane);
+        if (w == 1) fac1 = *reinterpret_cast<const f32x4 *>(records + rec * (BackRecord::units * 1024) + 16 * lane);
         f32x4 f[4] = {zero, zero, zero, zero}, z[4] = {zero, zero, zero, zero};
         {
             uint32_t y1[8];
@@ -369,6 +371,12 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                     if (j <= w) kept_row(kd.e(), 16 * j + c, pb, e1[j]);
             };
             load(0);
+            if constexpr (!MANY) put_rows();
+            if (w == 0) {
+                G[lane] = wave_scan<1>(static_cast<double>(clamp_decay(g1)), lane);
+                beta[lane] = b1;
+            }
+            if (w == 1) *reinterpret_cast<f32x4 *>(fac + 4 * lane) = fac1;
 #pragma unroll 1
             for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
                 bf16x8 ya[KP], ra[kNP], eb[4][kNP];
