@@ -53,14 +53,6 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
     const uint32_t dv_at = row_off<T>(pv, P, 4 * g, p);
     const Kept kd(a);
     const int nt0 = half * NT, kk0 = half * KS;
-    f32x4 S[NT];   // the gradient of the state after the chunk
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt0 + nt, g, r);
-            S[nt][r] = gr.dstate && p < P && n < n_of ? gr.dstate[(bh * P + p) * n_of + n] : 0.f;
-        }
     const int live = (len + kC - 1) / kC;
     St in(a, b, h, len, static_cast<const T *>(gr.dy) + row0, pv, p0, records + bh * chunks * rec_bytes, rec_bytes);
     if constexpr (DMA) {
@@ -86,6 +78,15 @@ delta_reverse(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int ch
     } else {
         if (live > 0) in.fetch(live - 1);
     }
+    // the gradient of the state after the chunk (the fifth wave has no columns)
+    f32x4 S[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = state_n(nt0 + nt, g, r);
+            S[nt][r] = gr.dstate && p < P && n < n_of ? gr.dstate[(bh * P + p) * n_of + n] : 0.f;
+        }
     // rows 32 half .. of a chunk's dR: written a chunk later, so that the wait for
     // the operands does not wait for them
     f32x4 late[2];

@@ -279,19 +279,6 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
     const uint32_t y_at = row_off<T>(ystep, P, 4 * g, p);
     const Kept kd(a);
     const int nt0 = half * NT, kk0 = half * KS;
-    f32x4 S[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int n = state_n(nt0 + nt, g, r);
-            if constexpr (MODE == kCarry)
-                S[nt][r] = n == unit_row ? 1.f : 0.f;
-            else if (sg.count > 1)
-                S[nt][r] = sg.starts[((bh * sg.count + seg) * sg.cols + p) * N + n];
-            else
-                S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
-        }
     const int all = (len + kC - 1) / kC, first = seg * sg.chunks;
     const int live = sg.chunks < all - first ? first + sg.chunks : all;   // the segment's end
     St in(a, b, h, len, static_cast<const T *>(a.v) + b * L * a.vs + h * P, a.vs, p0,
@@ -330,6 +317,25 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         }
     } else {
         if (first < live) in.fetch(first);
+    }
+    // (after the fifth wave has gone its way: it has no columns)
+    f32x4 S[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int n4 = state_n(nt0 + nt, g, 0);
+        if constexpr (MODE != kCarry)
+            if (sg.count > 1) {
+                S[nt] = *reinterpret_cast<const f32x4 *>(sg.starts + ((bh * sg.count + seg) * sg.cols + p) * N + n4);
+                continue;
+            }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = n4 + r;
+            if constexpr (MODE == kCarry)
+                S[nt][r] = n == unit_row ? 1.f : 0.f;
+            else
+                S[nt][r] = a.state && p < P && n < n_of ? a.state[(bh * P + p) * n_of + n] : 0.f;
+        }
     }
     // rows 32 half .. of a chunk's Y (KEEP: E): written a chunk later, so that the
     // wait for the operands does not wait for them
