@@ -338,17 +338,31 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             out[0] = *reinterpret_cast<const f32x4 *>(s);
             out[1] = *reinterpret_cast<const f32x4 *>(s + 16);
         };
+        // dY's, four columns in one load where the rows allow it
+        constexpr int words = VEC ? 2 * sizeof(T) : 8;
         const auto dy_row = [&](int pb, uint32_t *out) {
+            if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
-                out[j] = load_one(dyr, row_off<T>(dyr.stride, P, my, n), my, n, 0);
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t at = row_off<T>(dyr.stride, P, my, pb + 16 * j + 4 * g);
+                    if constexpr (sizeof(T) == 4)
+                        *reinterpret_cast<u32x4 *>(out + 4 * j) = bld16(dyr.r, at);
+                    else
+                        *reinterpret_cast<u32x2 *>(out + 2 * j) = bld8(dyr.r, at);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int n = pb + 16 * (j >> 2) + 4 * g + (j & 3);
+                    out[j] = load_one(dyr, row_off<T>(dyr.stride, P, my, n), my, n, 0);
+                }
             }
         };
         const auto dy_parts = [&](const uint32_t *y, bf16x8 *out) {
             float y8[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y8[j] = value_of<T>(y[j]);
+            for (int j = 0; j < 8; ++j)
+                y8[j] = words == 8 ? value_of<T>(y[j]) : value_of<T>(y[j >> 1] >> (16 * (j & 1)) & 0xFFFFu);
             split8<KP>(y8, out);
         };
         // this head's decays, steps and factors, on their way while the rows are put down
@@ -362,7 +376,7 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
         if (w == 1) fac1 = *reinterpret_cast<const f32x4 *>(records + rec * (BackRecord::units * 1024) + 16 * lane);
         f32x4 f[4] = {zero, zero, zero, zero}, z[4] = {zero, zero, zero, zero};
         {
-            uint32_t y1[8];
+            __attribute__((aligned(16))) uint32_t y1[words];
             f32x4 r1[2], e1[4][2];
             const auto load = [&](int pb) {
                 dy_row(pb, y1);
@@ -399,27 +413,26 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
         constexpr int pieces = 32 * N / 8 / 256;
         // piece i of this wave: columns 16 (w & 1) .. of the block, n of the pair of tiles i
         const auto pair = [&](int i) { return (w >> 1) + 2 * i; };
-        f32x4 s0[pieces][2], s1[pieces][2], r1[2], e1[2];
-        uint32_t y1[8];
-        const auto load_state = [&](size_t at, int pb, f32x4(*out)[2]) {
+        f32x4 st[pieces][2], r1[2];   // S0, then dS1; rows of dR, then of E
+        __attribute__((aligned(16))) uint32_t y1[words];
+        const auto load_state = [&](size_t at, int pb) {
 #pragma unroll
             for (int i = 0; i < pieces; ++i) {
                 const float *s = keep + at + kd.tile(pb + 16 * (w & 1), 2 * pair(i), lane);
-                out[i][0] = *reinterpret_cast<const f32x4 *>(s);
-                out[i][1] = *reinterpret_cast<const f32x4 *>(s + 256);
+                st[i][0] = *reinterpret_cast<const f32x4 *>(s);
+                st[i][1] = *reinterpret_cast<const f32x4 *>(s + 256);
             }
         };
         const auto load_first = [&](int pb) {
-            load_state(kd.s0(), pb, s0);
+            load_state(kd.s0(), pb);
             dy_row(pb, y1);
             kept_row(kd.dr(), my, pb, r1);
         };
         const auto load_second = [&](int pb) {
-            load_state(kd.s1(), pb, s1);
-            kept_row(kd.e(), my, pb, e1);
+            load_state(kd.s1(), pb);
+            kept_row(kd.e(), my, pb, r1);
         };
         load_first(0);
-        load_second(0);
         scan::lds_barrier();
         {
             f32x4 qkt[4] = {zero, zero, zero, zero}, kkt[4] = {zero, zero, zero, zero};
@@ -477,15 +490,17 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
         for (int nt = 0; nt < NT; ++nt) dq[nt] = ki[nt] = dk[nt] = zero;
 #pragma unroll 1
         for (int pb = 0; pb < static_cast<int>(kd.p64); pb += 32) {
-            const auto put = [&](const f32x4(*s)[2]) {
+            const auto mine = [&](int i, int q) {
+                return reinterpret_cast<bf16x8 *>(area + q * (Tile<N>::bytes / 2) +
+                                                  tile_at<N>(16 * (w & 1) + c, 4 * pair(i) + g));
+            };
+            const auto put = [&]() {
 #pragma unroll
                 for (int i = 0; i < pieces; ++i) {
                     bf16x8 x[kNP];
-                    split_tiles<kNP>(s[i][0], s[i][1], x);
+                    split_tiles<kNP>(st[i][0], st[i][1], x);
 #pragma unroll
-                    for (int q = 0; q < kNP; ++q)
-                        *reinterpret_cast<bf16x8 *>(area + q * (Tile<N>::bytes / 2) +
-                                                    tile_at<N>(16 * (w & 1) + c, 4 * pair(i) + g)) = x[q];
+                    for (int q = 0; q < kNP; ++q) *mine(i, q) = x[q];
                 }
             };
             const auto state = [&](int nt, bf16x8 *out) {
@@ -496,10 +511,8 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
             dy_parts(y1, ya);
             split_tiles<kNP>(r1[0], r1[1], ra);
             scan::lds_barrier();
-            put(s0);
-#pragma unroll
-            for (int i = 0; i < pieces; ++i) dot4 += s0[i][0] * s1[i][0] + s0[i][1] * s1[i][1];
-            if (pb + 32 < static_cast<int>(kd.p64)) load_first(pb + 32);
+            put();
+            load_second(pb);
             scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -509,10 +522,19 @@ delta_grads(DeltaLaunch a, DeltaGrads gr, const unsigned char *records, int chun
                 ki[nt] = mma_parts<kNP, kNP>(ra, s, ki[nt]);
                 if (nt & 1) __builtin_amdgcn_sched_barrier(0);
             }
-            split_tiles<kNP>(e1[0], e1[1], ra);
+            split_tiles<kNP>(r1[0], r1[1], ra);
+            // <S0, dS1> from S0's parts where this thread put them
+#pragma unroll
+            for (int i = 0; i < pieces; ++i)
+#pragma unroll
+                for (int q = kNP - 1; q >= 0; --q) {
+                    const bf16x8 x = *mine(i, q);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dot4[j & 3] += static_cast<float>(x[j]) * st[i][j >> 2][j & 3];
+                }
             scan::lds_barrier();
-            put(s1);
-            if (pb + 32 < static_cast<int>(kd.p64)) load_second(pb + 32);
+            put();
+            if (pb + 32 < static_cast<int>(kd.p64)) load_first(pb + 32);
             scan::lds_barrier();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
