@@ -13,6 +13,11 @@
 // step is a sum over the row or elementwise: 16-byte pieces where the rows allow
 // it (VEC), else values a stride apart, so that a wave's scalar loads are
 // contiguous.
+//
+// 32768 rows of 768 (bf16, residual f32): 352 MB in 69 us, 5.1 TB/s.  16384 rows of
+// 1536 (bf16): 252 MB in 50 us; the gradient 403 MB and 19 MB of partial sums in 104 us
+// (3.9 TB/s) and 5 more to add those: its vector instructions are the nearer bound, 80 %
+// of the issue slots.
 #include "delta.hpp"
 #include "m3_internal.hpp"
 #include "scan_common.hpp"

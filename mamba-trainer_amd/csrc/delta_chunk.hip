@@ -8,7 +8,10 @@ namespace {
 using namespace delta;
 
 // One workgroup a (sequence, head, chunk): the chunk's row factors, T and the
-// attention within the chunk.
+// attention within the chunk.  What the chunks' chain would else redo for every
+// column block of P is done once here and left as ready operands.  Near a copy's
+// rate: 8 x 2048 tokens, 12 heads (64, 128), bf16: 101 MB of q and k read and 97 of
+// records written in 46 us, 4.3 TB/s (BACK: 172 written in 56 us).
 template <typename T, int N, bool VEC, bool BACK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta_prep(DeltaLaunch a, unsigned char *records, int chunks) {
     constexpr int KP = Parts<T>::in, LP = kC + 4;
@@ -238,6 +241,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // second buffer while the one before is multiplied, Q to the buffer it has left.
 // KEEP is the backward's way in: no y, but the state before each chunk and its E
 // are kept.
+//
+// Bound by its own chain: a workgroup a CU, one chunk after another, each some
+// 5500 cycles of products that wait for each other (the matrix unit is busy 29 % of
+// them, vector instructions 35 %).  So what stood beside the chain was moved off
+// it, 8 x 2048 tokens, 12 heads (64, 128), bf16: pairs of waves a column tile instead of one
+// 149 -> 117 us, the fetch in a fifth wave 117 -> 92; KEEP 97 us.  Two workgroups
+// a CU on a CARRY pass take 1.9 times as long as one.
 //
 // Few sequences leave most CUs idle while their chunks pass one by one; then the
 // window is cut into segments that run side by side.  As S [P, N] passes through
@@ -528,7 +538,8 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
 
 // The state before each segment: one workgroup a (sequence, head, 16 rows of S),
 // a wave 16 columns, S_s Phi_s + Psi_s segment by segment in f32 (MFMA 16x16x4);
-// the next segment's Phi and Psi are on their way meanwhile.
+// the next segment's Phi and Psi are on their way meanwhile.  A chain of loads and
+// products: 20 us for ten segments of 12 heads (64, 128).
 template <int N>
 __global__ void __launch_bounds__(4 * N) delta_join(DeltaLaunch a, Segments sg) {
     constexpr int KS = N / 4;
@@ -573,10 +584,12 @@ __global__ void __launch_bounds__(4 * N) delta_join(DeltaLaunch a, Segments sg) 
     }
 }
 
-// Segments of a window, by the time its chunk passes take in chunks (an LDS-full
-// workgroup a CU, 256 CUs; each segment joined 3/4 of a chunk, the launches four).  Measured on MI355X, one
-// sequence of 12 heads (64, 128), bf16, with and without: 16384 tokens 334 against 828 us, 2048
-// 77 against 116; from 24 heads of 2048 tokens on a window stays whole.
+// Segments of a window, by the time its chunk passes take in chunks (256 CUs, a
+// workgroup each, as two together take the time of one after the other; each segment
+// joined 3/4 of a chunk, the launches four).  Measured on MI355X, one sequence of 12 heads
+// (64, 128), bf16, with and without: 16384 tokens 278 against 655 us, 4096 101 against
+// 173, 2048 70 against 97; 1024 tokens 58 either way, and two sequences of 2048 are left
+// whole (98).
 size_t segments_of(const DeltaLaunch &a) {
     const size_t chunks = chunks_of(a), heads = a.batch * a.heads, n = a.d_state <= 64 ? 64 : 128;
     const size_t tiles = (a.head_dim + kCols - 1) / kCols;
@@ -689,8 +702,9 @@ hipError_t delta::launch_delta_states(const DeltaLaunch &a, unsigned char *works
 
 // Against the recurrence token by token, which reads and writes the state once and
 // then takes its tokens one by one.  Measured on MI355X, heads of (64, 128) bf16,
-// recurrence and chunks: 96 heads 16 tokens 17.5 and 20 us a call, 8 tokens 16 and
-// 20; 1536 heads 16 tokens 65 and 120, growing by 3.4 a token against 0.3.
+// recurrence and chunks: 96 heads 16 tokens 17.2 and 19.7 us a call, 24 tokens 23.5
+// and 19.4; 1536 heads 16 tokens 61 and 118, 32 tokens 112 and 123, 48 tokens 165 and
+// 127.
 bool delta_chunk_wanted(const DeltaLaunch &a) {
     return a.d_state <= 128 && a.seq > (a.batch * a.heads >= 1024 ? 32u : 16u);
 }
