@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // of waves has sixteen columns, each half of the state's N: their halves of K S0^T
 // (and of Q S0^T) meet in LDS, then both form E, and each its half of S and of
 // Y's rows.  DMA: what is read first in a chunk (K, v, the record) goes to a
-// second buffer while the one before is multiplied, Q to the buffer it has left.
+// second buffer while the one before is multiplied, Q to the buffer it has left
+// (without Q: v and T to theirs).
 // KEEP is the backward's way in: no y, but the state before each chunk and its E
 // are kept.
 //
@@ -246,8 +247,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // 5500 cycles of products that wait for each other (the matrix unit is busy 29 % of
 // them, vector instructions 35 %).  So what stood beside the chain was moved off
 // it, 8 x 2048 tokens, 12 heads (64, 128), bf16: pairs of waves a column tile instead of one
-// 149 -> 117 us, the fetch in a fifth wave 117 -> 92; KEEP 97 us.  Two workgroups
-// a CU on a CARRY pass take 1.9 times as long as one.
+// 149 -> 117 us, the fetch in a fifth wave 117 -> 92.  The passes without outputs
+// fetch less: there the four waves do it (KEEP 97 -> 89 us), and as five waves of
+// their registers would not, two workgroups of four fit a CU (CARRY 162 -> 139 us at 16384
+// tokens of one sequence).
 //
 // Few sequences leave most CUs idle while their chunks pass one by one; then the
 // window is cut into segments that run side by side.  As S [P, N] passes through
@@ -258,13 +261,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && N == 128 ? 2 : 4) delta
 // (2 P + N) / P times the work, in segments' time.
 enum { kWindow, kKeep, kCarry };
 template <typename T, int N, bool VEC, int MODE, bool BACK>
-__global__ void __launch_bounds__((kChunkThreads<T, VEC>), (kDma<T, VEC> && MODE != kWindow ? 3 : 1))
+__global__ void __launch_bounds__((kChunkThreads<T, VEC, MODE != kWindow>), (kDma<T, VEC> && MODE != kWindow ? 2 : 1))
 delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kept, Segments sg) {
     constexpr bool KEEP = MODE == kKeep, Y = MODE == kWindow;
     constexpr int KP = Parts<T>::in, YP = Parts<T>::out, KS = N / 64, NT = N / 32;   // of this wave
     using R = Record<T>;
     constexpr size_t rec_bytes = (BACK ? BackRecord::units : R::units) * 1024;
-    using St = Stage<T, N, VEC, Y, Y ? R::units : R::p, 0>;
+    using St = Stage<T, N, VEC, Y, Y ? R::units : R::p, 0, !Y>;
     constexpr bool DMA = St::DMA;
     constexpr int BUFS = DMA ? 2 : 1;
     __shared__ __attribute__((aligned(1024))) typename St::Rows1 sk[BUFS];
@@ -293,34 +296,35 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
     const int live = sg.chunks < all - first ? first + sg.chunks : all;   // the segment's end
     St in(a, b, h, len, static_cast<const T *>(a.v) + b * L * a.vs + h * P, a.vs, p0,
           records + bh * chunks * rec_bytes, rec_bytes);
+    const auto first_half = [&](int ck) {
+        in.dma_k(sk[ck & 1], ck);
+        if constexpr (Y) {
+            in.dma_v(sv[ck & 1], ck);
+            in.template dma_rec<0, R::units>(sr[ck & 1].at, ck);
+        } else {
+            in.template dma_rec<0, 1>(ck & 1 ? odd_fac : sr[0].at, ck);
+        }
+    };
+    const auto second_half = [&](int ck) {
+        if constexpr (Y) {
+            in.dma_q(sq, ck);
+        } else {
+            in.dma_v(sv[0], ck);
+            in.template dma_rec<R::t, R::p>(sr[0].at, ck);
+        }
+    };
     if constexpr (DMA) {
-        if (wave == 4) {
-            const auto first_half = [&](int ck) {
-                in.dma_k(sk[ck & 1], ck);
-                if constexpr (Y) {
-                    in.dma_v(sv[ck & 1], ck);
-                    in.template dma_rec<0, R::units>(sr[ck & 1].at, ck);
-                } else {
-                    in.template dma_rec<0, 1>(ck & 1 ? odd_fac : sr[0].at, ck);
-                }
-            };
-            const auto second_half = [&](int ck) {
-                if constexpr (Y) {
-                    in.dma_q(sq, ck);
-                } else {
-                    in.dma_v(sv[0], ck);
-                    in.template dma_rec<R::t, R::p>(sr[0].at, ck);
-                }
-            };
+        if (Y ? wave == 4 : true)
             if (first < live) {
                 first_half(first);
                 second_half(first);
             }
+        if (Y && wave == 4) {
             for (int ck = first; ck < live; ++ck) {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 scan::lds_barrier();   // the chunk is there, the one before is done with
                 if (ck + 1 < live) first_half(ck + 1);
-                scan::lds_barrier();   // Q, or v and T, are done with
+                scan::lds_barrier();   // Q is done with
                 if (ck + 1 < live) second_half(ck + 1);
             }
             return;
@@ -384,6 +388,7 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
         const unsigned char *rec = sr[TWO ? now : 0].at;
         f32x4 e[4];
         if constexpr (DMA) {
+            if constexpr (!Y) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             scan::lds_barrier();
         } else {
             __syncthreads();
@@ -425,6 +430,8 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             } else {
                 if constexpr (DMA) in.values(sv[TWO ? now : 0], e);
             }
+            if constexpr (DMA && !Y)
+                if (kk == 0 && ck + 1 < live) first_half(ck + 1);
             __builtin_amdgcn_sched_barrier(0);
             if (kk + 1 < KS) split_tiles<kNP>(S[2 * kk + 2], S[2 * kk + 3], sp[(kk + 1) & 1]);
             mma_rows<4, KP, kNP>(kf[kk & 1], sp[kk & 1], ks);
@@ -445,6 +452,8 @@ delta_chunks(DeltaLaunch a, const unsigned char *records, int chunks, float *kep
             }
         tri_load<kNP>(rec + R::t * 1024, lane, t4, t2, false);
         scan::lds_barrier();
+        if constexpr (DMA && !Y)
+            if (ck + 1 < live) second_half(ck + 1);   // v and T are done with
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             ks[i] += meet[wave ^ 1][i][lane];
@@ -585,11 +594,11 @@ __global__ void __launch_bounds__(4 * N) delta_join(DeltaLaunch a, Segments sg) 
 }
 
 // Segments of a window, by the time its chunk passes take in chunks (256 CUs, a
-// workgroup each, as two together take the time of one after the other; each segment
-// joined 3/4 of a chunk, the launches four).  Measured on MI355X, one sequence of 12 heads
-// (64, 128), bf16, with and without: 16384 tokens 278 against 655 us, 4096 101 against
-// 173, 2048 70 against 97; 1024 tokens 58 either way, and two sequences of 2048 are left
-// whole (98).
+// workgroup each; the carry pass is counted alike, though two fit and take 1.4 times
+// one's time; each segment joined 3/4 of a chunk, the launches four).  Measured on MI355X,
+// one sequence of 12 heads (64, 128), bf16, with and without: 16384 tokens 255 against 655
+// us, 4096 94 against 173, 2048 66 against 97; 1024 tokens 58 either way, and two
+// sequences of 2048 are left whole (98).
 size_t segments_of(const DeltaLaunch &a) {
     const size_t chunks = chunks_of(a), heads = a.batch * a.heads, n = a.d_state <= 64 ? 64 : 128;
     const size_t tiles = (a.head_dim + kCols - 1) / kCols;
@@ -651,13 +660,14 @@ hipError_t launch(const DeltaLaunch &a, unsigned char *workspace, size_t segment
             const unsigned tiles = static_cast<unsigned>(BACK ? kept_cols(a) : (a.head_dim + kCols - 1) / kCols);
             const auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
-                constexpr unsigned threads = kChunkThreads<T, VEC>;
+                constexpr unsigned threads = kChunkThreads<T, VEC, MODE != kWindow>;
+                constexpr unsigned carry_threads = kChunkThreads<T, VEC, true>;
                 hipLaunchKernelGGL((delta_prep<T, N, VEC, BACK>), dim3(heads * chunks), dim3(256), 0, s, a, workspace,
                                    chunks);
                 if (plan.count > 1) {
                     const dim3 carry(heads * static_cast<unsigned>(plan.count),
                                      static_cast<unsigned>((plan.cols + N) / kCols));
-                    hipLaunchKernelGGL((delta_chunks<T, N, VEC, kCarry, BACK>), carry, dim3(threads), 0, s, a, workspace,
+                    hipLaunchKernelGGL((delta_chunks<T, N, VEC, kCarry, BACK>), carry, dim3(carry_threads), 0, s, a, workspace,
                                        chunks, kept, sg);
                     hipLaunchKernelGGL((delta_join<N>), dim3(heads, static_cast<unsigned>(plan.cols / 16)), dim3(4 * N), 0,
                                        s, a, sg);

@@ -319,11 +319,12 @@ constexpr int kCols = 32;
 // The fetch of a chunk's operands to LDS: K, Q, a tile of v (or dy), and UNITS
 // kilobytes of its record (unit u > 0 from kilobyte u + GAP).  bf16 with aligned
 // rows (DMA): straight from memory, by a fifth wave that does nothing else (issuing
-// them stalls a wave some 100 cycles a kilobyte).  Other inputs become their bf16
-// parts on the way, through registers; v stays there.
+// them stalls a wave some 100 cycles a kilobyte), or by the four waves themselves
+// (SELF).  Other inputs become their bf16 parts on the way, through registers; v stays
+// there.
 template <typename T, bool VEC> constexpr bool kDma = VEC && std::is_same<T, bf16_t>::value;
-template <typename T, bool VEC> constexpr unsigned kChunkThreads = kDma<T, VEC> ? 320 : 256;
-template <typename T, int N, bool VEC, bool WITHQ, int UNITS, int GAP>
+template <typename T, bool VEC, bool SELF = false> constexpr unsigned kChunkThreads = kDma<T, VEC> && !SELF ? 320 : 256;
+template <typename T, int N, bool VEC, bool WITHQ, int UNITS, int GAP, bool SELF = false>
 struct Stage {
     static constexpr int KP = Parts<T>::in;
     static constexpr bool DMA = kDma<T, VEC>;
@@ -334,8 +335,9 @@ struct Stage {
     const T *kp, *qp, *vp;              // the sequence's rows of this head
     size_t ks, qs, vs, rec_bytes;
     const unsigned char *rec;           // the sequence's records
-    int len, n_of, P, wave, w, lane;    // wave: 4 is the DMA's; w: its tile of columns
-    uint32_t dk[4], dq[4], dv[4];       // DMA: places in a kilobyte, by kilobyte modulo 4
+    int len, n_of, P, wave, w, lane;    // wave: 4 is the DMA's, unless SELF; w: its tile of columns
+    static constexpr int own = SELF ? 1 : 4;
+    uint32_t dk[own], dq[own], dv[own];   // DMA: places in a kilobyte, by kilobyte modulo 4
     int kt, kn, vt, vn;                 // else: this thread's places
     uint32_t k_at, q_at, v_at;
     Eight<T> k8[pieces], q8[WITHQ ? pieces : 1];
@@ -366,10 +368,10 @@ struct Stage {
         vn = p0 + 16 * w + (lane & 15);
         if constexpr (DMA) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dk[i] = dma_at<T, N>(ks, n_of, 0, i, lane);
-                dq[i] = dma_at<T, N>(qs, n_of, 0, i, lane);
-                dv[i] = dma_at<T, kCols>(vs, P, p0, i, lane);
+            for (int i = 0; i < own; ++i) {
+                dk[i] = dma_at<T, N>(ks, n_of, 0, nth(i), lane);
+                dq[i] = dma_at<T, N>(qs, n_of, 0, nth(i), lane);
+                dv[i] = dma_at<T, kCols>(vs, P, p0, nth(i), lane);
             }
         } else {
             k_at = row_off<T>(ks, n_of, kt, kn);
@@ -377,6 +379,7 @@ struct Stage {
             v_at = row_off<T>(vs, P, vt, vn);
         }
     }
+    __device__ __forceinline__ int nth(int i) const { return SELF ? wave : i; }
     __device__ __forceinline__ rsrc_t record(int ck) const { return make_rsrc(rec + ck * rec_bytes, static_cast<uint32_t>(rec_bytes)); }
     static __device__ __forceinline__ constexpr int unit(int u) { return u == 0 ? 0 : u + GAP; }
     __device__ __forceinline__ Rows<T, VEC> rows_of(const T *p, size_t stride, int ck, int width) const {
@@ -386,23 +389,26 @@ struct Stage {
     __device__ __forceinline__ void dma_k(Rows1 &to, int ck) const {
         const Rows<T, VEC> rows = rows_of(kp, ks, ck, n_of);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma_tile<N>(rows, dk[i], to.part[0], i);
+        for (int i = 0; i < own; ++i) dma_tile<N>(rows, dk[i], to.part[0], nth(i));
     }
     __device__ __forceinline__ void dma_q(Rows1 &to, int ck) const {
         const Rows<T, VEC> rows = rows_of(qp, qs, ck, n_of);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma_tile<N>(rows, dq[i], to.part[0], i);
+        for (int i = 0; i < own; ++i) dma_tile<N>(rows, dq[i], to.part[0], nth(i));
     }
     __device__ __forceinline__ void dma_v(V &to, int ck) const {
         const Rows<T, VEC> rows = rows_of(vp, vs, ck, P);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma_tile<kCols>(rows, dv[i], to.at, i);
+        for (int i = 0; i < own; ++i) dma_tile<kCols>(rows, dv[i], to.at, nth(i));
     }
     template <int FROM, int END>   // kilobytes FROM .. of the record, to where its first would lie at `to`
     __device__ __forceinline__ void dma_rec(unsigned char *to, int ck) const {
         const rsrc_t r = record(ck);
 #pragma unroll
-        for (int u = FROM; u < END; ++u) scan::lds_dma16(r, scan::lds_addr(to + u * 1024), unit(u) * 1024 + lane * 16);
+        for (int i = 0; i < (END - FROM + 4 / own - 1) / (4 / own); ++i) {
+            const int u = FROM + (SELF ? wave + 4 * i : i);
+            if (u < END) scan::lds_dma16(r, scan::lds_addr(to + u * 1024), unit(u) * 1024 + lane * 16);
+        }
     }
     __device__ __forceinline__ void fetch(int ck) {
         const Rows<T, VEC> kr = rows_of(kp, ks, ck, n_of), qr = rows_of(qp, qs, ck, n_of), vr = rows_of(vp, vs, ck, P);
